@@ -31,7 +31,9 @@ NAME = "harp_b200_C"
 SOURCES = [
     "ops.cpp",
     "gemm_sm100.cu",
+    "gemm_s8_sm100.cu",
     "elementwise.cu",
+    "quant.cu",
     "attention_sm100.cu",
     "comm.cu",
     "runtime.cpp",

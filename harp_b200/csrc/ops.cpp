@@ -57,6 +57,18 @@ void adamw_list(at::TensorList params, at::TensorList grads, at::TensorList exp_
 void philox_uniform(at::Tensor& out, int64_t seed, int64_t offset, double lo, double hi);
 void rowdot(const at::Tensor& a, const at::Tensor& b, int64_t H, int64_t Dh, int64_t S, at::Tensor& out);
 
+// quant.cu
+std::tuple<at::Tensor, at::Tensor> quant_rows(const at::Tensor& x);
+std::tuple<at::Tensor, at::Tensor> swiglu_quant(const at::Tensor& gu);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rmsnorm_mod_quant(
+    const at::Tensor& x, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& scale,
+    const c10::optional<at::Tensor>& shift, int64_t rows_per_batch, double eps,
+    const c10::optional<at::Tensor>& residual, const c10::optional<at::Tensor>& gate);
+at::Tensor dequant_rows(const at::Tensor& q, const at::Tensor& s, bool f32);
+// gemm_s8_sm100.cu
+void gemm_s8(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, const at::Tensor& sb,
+             const c10::optional<at::Tensor>& bias, at::Tensor& C, at::Tensor& err);
+
 namespace {
 
 // Per-device error word used by the compat ops (which have no err argument).
@@ -240,6 +252,12 @@ TORCH_LIBRARY(harp, m) {
         "float beta1, float beta2, float eps, float wd, int step, float grad_scale, Tensor? hyper=None) -> ()");
   m.def("philox_uniform(Tensor(a!) out, int seed, int offset, float lo, float hi) -> ()");
   m.def("rowdot(Tensor a, Tensor b, int H, int Dh, int S, Tensor(a!) out) -> ()");
+  m.def("quant_rows(Tensor x) -> (Tensor, Tensor)");
+  m.def("swiglu_quant(Tensor gu) -> (Tensor, Tensor)");
+  m.def("rmsnorm_mod_quant(Tensor x, Tensor? w, Tensor? scale, Tensor? shift, int rows_per_batch, float eps, "
+        "Tensor? residual, Tensor? gate) -> (Tensor, Tensor, Tensor)");
+  m.def("dequant_rows(Tensor q, Tensor s, bool f32) -> Tensor");
+  m.def("gemm_s8(Tensor A, Tensor sa, Tensor B, Tensor sb, Tensor? bias, Tensor(a!) C, Tensor(b!) err) -> ()");
   m.def("launch_count() -> int");
   m.def("add_launch_count(int n) -> ()");
   m.def("reset_launch_count() -> ()");
@@ -268,6 +286,11 @@ TORCH_LIBRARY_IMPL(harp, CUDA, m) {
   m.impl("adamw_flat", &harp::adamw_flat);
   m.impl("philox_uniform", &harp::philox_uniform);
   m.impl("rowdot", &harp::rowdot);
+  m.impl("quant_rows", &harp::quant_rows);
+  m.impl("swiglu_quant", &harp::swiglu_quant);
+  m.impl("rmsnorm_mod_quant", &harp::rmsnorm_mod_quant);
+  m.impl("dequant_rows", &harp::dequant_rows);
+  m.impl("gemm_s8", &harp::gemm_s8);
 }
 
 TORCH_LIBRARY_IMPL(harp, CompositeExplicitAutograd, m) {

@@ -395,6 +395,122 @@ def gate_bwd(dy, a, gate, rows_per_batch, want_bias=True):
     return da.to(dy.dtype), dgate, dbias
 
 
+# ---------------------------------------------------------------------------
+# 8-bit integer rows and their GEMM (inference: no gradient passes the rounding)
+# ---------------------------------------------------------------------------
+_INT8_MIN_SCALE = 2.0 ** -126
+
+
+def _rows8(y: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    amax = y.abs().amax(1)
+    s = (amax * (1.0 / 127.0)).clamp_min(_INT8_MIN_SCALE)
+    q = torch.round(y * (1.0 / s)[:, None])
+    bad = ~(amax < float("inf"))
+    q = torch.where(bad[:, None], torch.zeros_like(q), q).clamp(-127, 127).to(torch.int8)
+    return q, torch.where(bad, torch.full_like(s, float("nan")), s)
+
+
+def _check_rows(x: torch.Tensor, op: str) -> None:
+    if x.dtype not in (torch.bfloat16, torch.float32) or x.dim() != 2 or x.shape[1] < 1:
+        raise RuntimeError(f"{op}: a 2-D bf16 or fp32 tensor with at least one column is required")
+
+
+def quant_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows of ``x`` [R, D] (bf16 or fp32) in 8 bits: ``(q int8 [R, D], s fp32 [R])`` with
+    ``s = max(max|x| / 127, 2^-126)`` and ``q = x / s`` rounded half to even; ``q * s`` is
+    within ``s / 2`` of ``x``.  For activations a row is a token, for a weight [N, K] an
+    output channel.  A row holding a NaN or an infinity has ``s = NaN``, ``q = 0``.  On CUDA the
+    rows of ``q`` start on 16-byte boundaries (row stride D rounded up to 16), as
+    :func:`gemm_s8` reads them fastest."""
+    if _cuda(x):
+        return torch.ops.harp.quant_rows(x)
+    _check_rows(x, "quant_rows")
+    return _rows8(x.float())
+
+
+def dequant_rows(q: torch.Tensor, s: torch.Tensor, dtype=torch.bfloat16) -> torch.Tensor:
+    """``q * s`` of :func:`quant_rows` in bf16 or fp32."""
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise RuntimeError(f"dequant_rows: bf16 or fp32 output, not {dtype}")
+    if _cuda(q):
+        return torch.ops.harp.dequant_rows(q, s, dtype == torch.float32)
+    return (q.float() * s[:, None]).to(dtype)
+
+
+def swiglu_quant(gu: torch.Tensor, F_: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``quant_rows(silu(g) * u)`` of ``gu = [g | u]`` [R, 2 F] without storing the product."""
+    if gu.dim() != 2 or gu.shape[1] != 2 * F_:
+        raise RuntimeError(f"swiglu_quant: gu must be [R, {2 * F_}], got {tuple(gu.shape)}")
+    if _cuda(gu):
+        return torch.ops.harp.swiglu_quant(gu)
+    _check_rows(gu, "swiglu_quant")
+    g, u = gu[:, :F_].float(), gu[:, F_:].float()
+    return _rows8(torch.nn.functional.silu(g) * u)
+
+
+def rmsnorm_mod_quant(x: torch.Tensor, w: Optional[torch.Tensor], scale: Optional[torch.Tensor],
+                      shift: Optional[torch.Tensor], rows_per_batch: int, eps: float,
+                      residual: Optional[torch.Tensor] = None,
+                      gate: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Residual addition, RMSNorm, modulation and 8-bit rows in one pass: ``(q, s, h)`` with
+
+      h = residual + gate[b] * x                       (h is x without a residual)
+      y = h * rsqrt(mean(h^2) + eps) * w * (1 + scale[b]) + shift[b]
+      (q, s) as :func:`quant_rows` of y
+
+    ``x`` and ``residual`` are [R, D] bf16 or fp32, the vectors have x's type: ``w`` [D];
+    ``scale``, ``shift``, ``gate`` [B, D] with ``B * rows_per_batch == R``.  ``h`` is rounded to
+    x's type when stored; the norm reads it before that rounding."""
+    if _cuda(x):
+        q, s, h = torch.ops.harp.rmsnorm_mod_quant(x, w, scale, shift, rows_per_batch, eps, residual, gate)
+        return q, s, (x if h is None else h)
+    _check_rows(x, "rmsnorm_mod_quant")
+    if gate is not None and residual is None:
+        raise RuntimeError("rmsnorm_mod_quant: gate needs a residual")
+    xf = x.float()
+    h = x
+    if residual is not None:
+        if gate is not None:
+            xf = _bcast(gate.float(), rows_per_batch) * xf
+        xf = residual.float() + xf
+        h = xf.to(x.dtype)
+    y = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
+    if w is not None:
+        y = y * w.float()
+    if scale is not None:
+        y = y * (1 + _bcast(scale.float(), rows_per_batch))
+    if shift is not None:
+        y = y + _bcast(shift.float(), rows_per_batch)
+    q, s = _rows8(y)
+    return q, s, h
+
+
+def gemm_s8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, *,
+            bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+            out_dtype=torch.bfloat16) -> torch.Tensor:
+    """``(a @ b.T) * a_scale[:, None] * b_scale[None, :] + bias`` with ``a`` [M, K] and ``b`` [N, K]
+    in int8 and exact 32-bit integer sums (K <= 131071); bf16 or fp32 result.
+
+    The operands come from the quantisers above.  Their rows may have any stride; the
+    tensor-core kernels take operands whose rows start on 16-byte boundaries."""
+    M, N = a.shape[0], b.shape[0]
+    if out is None:
+        out = torch.empty(M, N, device=a.device, dtype=out_dtype)
+    if _cuda(a):
+        torch.ops.harp.gemm_s8(a, a_scale, b, b_scale, bias, out, errors.word(a.device))
+        return out
+    if a.dtype != torch.int8 or b.dtype != torch.int8 or a.shape[1] != b.shape[1]:
+        raise RuntimeError("gemm_s8: int8 operands [M, K] and [N, K] are required")
+    if a.shape[1] > 131071:
+        raise RuntimeError(f"gemm_s8: K = {a.shape[1]} could overflow the 32-bit sums (at most 131071)")
+    acc = (a.double() @ b.double().t()).float()  # the integer sum, exact in fp64
+    acc = acc * a_scale[:, None] * b_scale[None, :]
+    if bias is not None:
+        acc = acc + bias.float()
+    out.copy_(acc.to(out.dtype))
+    return out
+
+
 def lse_ld(S: int) -> int:
     """Row stride of the per-(batch, head) LSE / delta buffers: S rounded up to a key tile."""
     return (S + 127) // 128 * 128
