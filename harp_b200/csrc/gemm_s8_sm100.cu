@@ -4,8 +4,18 @@
 //
 // The integer sum is exact (K <= 131071 keeps 128 * 128 * K below 2^31), so the
 // result is one rounding of the sum to fp32, two products and an addition, and
-// does not depend on the order of the K loop.
+// does not depend on the order of the K loop, its split or the kernel chosen.
+//
+// Three kernels:
+//   gemm_s8_pair  CTA pairs (cta_group::2), persistent over 256 x BN tiles: many
+//                 tokens and many channels; bound by the tensor pipe
+//   gemm_s8_rows  128 channels x up to 256 tokens a CTA, the K loop split over a
+//                 cluster that adds its integer sums through distributed shared
+//                 memory: few tokens (down to one) or few channels, where the
+//                 weights' bytes and the latency count
+//   gemm_s8_simt  CUDA cores, for operands TMA cannot address
 #include "common.cuh"
+#include "gemm_common.cuh"
 #include "gemm_sm100.h"
 
 #include <ATen/ATen.h>
@@ -41,6 +51,490 @@ __device__ __forceinline__ float bias_at(const S8Args& a, int n) {
                     : __bfloat162float(reinterpret_cast<const bf16*>(a.bias)[n]);
 }
 
+// ---------------------------------------------------------------------------
+// tcgen05 kind::i8: signed 8-bit operands, 32-bit integer accumulators.  One MMA
+// covers K = 32 (32 bytes), so the K-major shared-memory layout and its
+// descriptors are those of the bf16 kernels byte for byte.
+// ---------------------------------------------------------------------------
+// Instruction descriptor: [4,6) D format (2 = s32), [7,10) A format and [10,13) B
+// format (1 = signed 8-bit), [17,23) N>>3, [24,29) M>>4; both operands K-major.
+__host__ __device__ constexpr uint32_t make_idesc_s8(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_s8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  HARP_CHECK_TMEM(d_tmem, (int)(((idesc >> 17) & 0x3Fu) << 3), 215);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_s8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  HARP_CHECK_TMEM(d_tmem, (int)(((idesc >> 17) & 0x3Fu) << 3), 216);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---------------------------------------------------------------------------
+// CTA-pair kernel.  The same pipeline as the bf16 pair kernel (gemm_sm100.cu):
+// each CTA stages its own 128 rows of A and BN/2 rows of B, the leader issues
+// M = 256 MMAs, two accumulators let the epilogue of one tile run under the MMAs
+// of the next.  A stage is 256 deep in K (two 128-byte swizzle atoms a row), the
+// same bytes as the bf16 kernel's 128, at twice the arithmetic.
+//
+// Epilogue: each warp scales its 32 rows 128 bytes at a time, lays them out in
+// shared memory and one lane stores the block with TMA (whole 128-byte lines;
+// out of range rows and columns are dropped by the map).  A C that TMA cannot
+// address is written from the same buffer, a row of the block at a time.
+// ---------------------------------------------------------------------------
+constexpr int kThreads = 192;
+constexpr int kStageK = 256;
+
+template <int BN>
+struct PairCfg {
+  static constexpr int A_ATOM = 128 * 128;       // 128 rows x one 128-byte atom
+  static constexpr int B_ATOM = (BN / 2) * 128;
+  static constexpr int A_BYTES = A_ATOM * (kStageK / 128);
+  static constexpr int B_BYTES = B_ATOM * (kStageK / 128);
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGING = 4 * 2 * 4096;   // 4 epilogue warps x 2 buffers x (32 rows x 128 bytes)
+  static constexpr int VECS = 2 * BN * 4;        // the tile's channel scales and bias
+  static constexpr int STAGES = (232448 - 256 - STAGING - VECS) / STAGE_BYTES;
+  static constexpr int TMEM_COLS = (2 * BN <= 256) ? 256 : 512;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + STAGING + VECS + 256;
+  static_assert(STAGES >= 3 && STAGES <= 8 && SMEM_BYTES <= 232448, "pair GEMM stages");
+};
+
+__device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+template <int BN, typename OUT>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_s8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                 const __grid_constant__ CUtensorMap tmC, const S8Args args, int c_tma) {
+  using C_ = PairCfg<BN>;
+  constexpr int CW = 128 / (int)sizeof(OUT);  // columns of one 128-byte block
+  extern __shared__ __align__(1024) uint8_t smem[];  // swizzle atoms start on 1024-byte boundaries
+  uint8_t* smem_a = smem;
+  uint8_t* smem_b = smem + C_::STAGES * C_::A_BYTES;
+  uint8_t* staging = smem + C_::STAGES * C_::STAGE_BYTES;
+  float* vecs = reinterpret_cast<float*>(staging + C_::STAGING);  // channel scales [BN], bias [BN]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + C_::STAGING + C_::VECS);
+  uint64_t* full_bar = bars;                         // [STAGES] (leader's are used)
+  uint64_t* empty_bar = bars + C_::STAGES;           // [STAGES]
+  uint64_t* tfull_bar = bars + 2 * C_::STAGES;       // [2]
+  uint64_t* tempty_bar = bars + 2 * C_::STAGES + 2;  // [2] (leader's are used)
+  uint64_t* drain_bar = bars + 2 * C_::STAGES + 4;   // [1]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C_::STAGES + 5);
+
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  const uint32_t rank = cluster_rank();  // 0 = leader
+  const int num_m = (args.M + 255) / 256;
+  const int num_n = (args.N + BN - 1) / BN;
+  const int num_tiles = num_m * num_n;
+  const int num_kb = (args.K + kStageK - 1) / kStageK;
+  const int pair = blockIdx.x / 2, npairs = gridDim.x / 2;
+  int* err = args.err;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C_::STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull_bar[i], 1);
+      mbar_init(&tempty_bar[i], 8);
+    }
+    mbar_init(drain_bar, 1);
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    if (c_tma) tma_prefetch_desc(&tmC);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, C_::TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs' barriers exist and the paired TMEM is allocated
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ---------------- TMA producer (both CTAs) ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued[C_::STAGES] = {};
+      bool ok = true;
+      const uint32_t fb0 = peer_addr(smem_u32(&full_bar[0]), 0);  // the leader's barriers
+      for (int t = pair; t < num_tiles && ok; t += npairs) {
+        int mt, nt;
+        tile_coords(t, num_m, num_n, mt, nt);
+        const int m0 = mt * 256 + (int)rank * 128, n0 = nt * BN + (int)rank * (BN / 2);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1, err, 61)) { ok = false; break; }
+          const uint32_t fb = fb0 + stage * 8;
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * C_::STAGE_BYTES);
+#pragma unroll
+          for (int h = 0; h < kStageK / 128; ++h) {
+            const int k0 = kb * kStageK + h * 128;
+            tma_load_2d_pair(smem_a + stage * C_::A_BYTES + h * C_::A_ATOM, &tmA, fb, k0, m0);
+            tma_load_2d_pair(smem_b + stage * C_::B_BYTES + h * C_::B_ATOM, &tmB, fb, k0, n0);
+          }
+          issued[stage]++;
+          if (++stage == C_::STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      // this CTA's copies land before it can pass the final cluster barrier:
+      // the stage's empty barrier turns once the leader consumed it
+      for (int s = 0; s < C_::STAGES; ++s)
+        if (issued[s] > 0) mbar_wait_drain(&empty_bar[s], (uint32_t)((issued[s] - 1) & 1));
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (leader CTA) ----------------
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = make_idesc_s8(256, BN);
+      int stage = 0;
+      uint32_t phase = 0;
+      int local = 0;
+      bool ok = true;
+      for (int t = pair; t < num_tiles && ok; t += npairs, ++local) {
+        const int acc = local & 1;
+        const uint32_t acc_phase = (local >> 1) & 1;
+        if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1, err, 62)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, err, 63)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem_a + stage * C_::A_BYTES);
+          const uint32_t sb = smem_u32(smem_b + stage * C_::B_BYTES);
+#pragma unroll
+          for (int kk = 0; kk < kStageK / 32; ++kk) {
+            const int h = kk / 4, r = kk % 4;
+            const uint64_t adesc = make_sdesc(sa + h * C_::A_ATOM + r * 32, 16, 1024, kLayoutSw128);
+            const uint64_t bdesc = make_sdesc(sb + h * C_::B_ATOM + r * 32, 16, 1024, kLayoutSw128);
+            mma_s8_pair(d_tmem, adesc, bdesc, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+          }
+          const uint32_t eb = smem_u32(&empty_bar[stage]);
+          mma_commit_pair(eb);
+          mma_commit_pair(peer_addr(eb, 1));
+          if (++stage == C_::STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        const uint32_t tf = smem_u32(&tfull_bar[acc]);
+        mma_commit_pair(tf);
+        mma_commit_pair(peer_addr(tf, 1));
+      }
+      const uint32_t db = smem_u32(drain_bar);
+      mma_commit_pair(db);
+      mma_commit_pair(peer_addr(db, 1));
+    }
+    // both CTAs: the pair's MMAs are done before the paired TMEM goes away
+    if (lane == 0) mbar_wait_drain(drain_bar, 0);
+  } else {
+    // ---------------- epilogue (warps 2..5, both CTAs) ----------------
+    const int quarter = warp & 3;
+    const int et = threadIdx.x - 64;
+    uint8_t* const stage_out = staging + (warp - 2) * 8192;
+    int local = 0, nbuf = 0;
+    bool ok = true;  // after a failed wait the warp only keeps meeting the others at the barriers
+    const uint32_t te_leader[2] = {peer_addr(smem_u32(&tempty_bar[0]), 0), peer_addr(smem_u32(&tempty_bar[1]), 0)};
+    for (int t = pair; t < num_tiles; t += npairs, ++local) {
+      int mt, nt;
+      tile_coords(t, num_m, num_n, mt, nt);
+      const int acc = local & 1;
+      const uint32_t acc_phase = (local >> 1) & 1;
+      const int mw = mt * 256 + (int)rank * 128 + quarter * 32;  // the warp's first row
+      const float sa = mw + lane < args.M ? args.sa[mw + lane] : 0.f;
+      // this tile's channel scales and bias, once every warp is done with the last tile's
+      if (local > 0) epilogue_barrier();
+      for (int j = et; j < BN; j += 128) {
+        const int n = nt * BN + j;
+        vecs[j] = n < args.N ? args.sb[n] : 0.f;
+        vecs[BN + j] = n < args.N ? bias_at(args, n) : 0.f;
+      }
+      epilogue_barrier();
+      ok = ok && mbar_wait(&tfull_bar[acc], acc_phase, err, 64);
+      if (!ok) continue;
+      tc_fence_after();
+      const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
+#pragma unroll 1
+      for (int c = 0; c < BN / CW; ++c) {
+        const int n0 = nt * BN + c * CW;
+        if (n0 >= args.N || mw >= args.M) break;
+        uint8_t* const buf = stage_out + (nbuf & 1) * 4096;
+        ++nbuf;
+        if (lane == 0) bulk_wait_read<1>();  // the store that last read this buffer is done with it
+        __syncwarp();
+        uint8_t* const brow = buf + lane * 128;
+#pragma unroll
+        for (int g = 0; g < CW / 32; ++g) {
+          uint32_t v[32];
+          tmem_ld32(tbase + c * CW + g * 32, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j4 = 0; j4 < 8; ++j4) {
+            const float4 s4 = *reinterpret_cast<const float4*>(vecs + c * CW + g * 32 + j4 * 4);
+            const float4 b4 = *reinterpret_cast<const float4*>(vecs + BN + c * CW + g * 32 + j4 * 4);
+            const float x0 = fmaf((float)(int)v[4 * j4 + 0] * sa, s4.x, b4.x);
+            const float x1 = fmaf((float)(int)v[4 * j4 + 1] * sa, s4.y, b4.y);
+            const float x2 = fmaf((float)(int)v[4 * j4 + 2] * sa, s4.z, b4.z);
+            const float x3 = fmaf((float)(int)v[4 * j4 + 3] * sa, s4.w, b4.w);
+            if constexpr (sizeof(OUT) == 2) {
+              v[2 * j4] = pack_bf16x2(x0, x1);
+              v[2 * j4 + 1] = pack_bf16x2(x2, x3);
+            } else {
+              *reinterpret_cast<float4*>(brow + ((j4 ^ (lane & 7)) << 4)) = make_float4(x0, x1, x2, x3);
+            }
+          }
+          if constexpr (sizeof(OUT) == 2) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<uint4*>(brow + (((g * 4 + q) ^ (lane & 7)) << 4)) =
+                  make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          }
+        }
+        if (c_tma) {
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmC, buf, n0, mw);
+            bulk_commit();
+          }
+        } else {
+          __syncwarp();
+          const int rows = min(32, args.M - mw), cols = min(CW, args.N - n0);
+          for (int r = 0; r < rows; ++r) {
+            OUT* crow = reinterpret_cast<OUT*>(args.C) + (long)(mw + r) * args.ldc + n0;
+#pragma unroll
+            for (int j = lane; j < CW; j += 32) {
+              const int byte = j * (int)sizeof(OUT);
+              if (j < cols)
+                crow[j] = *reinterpret_cast<const OUT*>(buf + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
+            }
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(te_leader[acc]);
+    }
+    if (lane == 0) bulk_wait_read<0>();  // the staging buffers outlive the stores that read them
+  }
+
+  tc_fence_before();
+  cluster_sync_all();  // neither CTA frees its half of the pair's TMEM while the other still works
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, C_::TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few tokens or few channels.  A CTA multiplies 128 channels (the MMA's M) by NT
+// tokens (its N) over its share of K; a cluster of `splits` CTAs along x covers
+// K.  Each CTA of a split tile leaves its integer sums in its shared memory, the
+// cluster meets, and rank r adds and stores tokens r*NT/splits onwards, read from
+// every rank's memory: one launch, no workspace, and the same sum in any order.
+// ---------------------------------------------------------------------------
+template <int NT>
+struct RowsCfg {
+  static constexpr int A_BYTES = 128 * 128;
+  static constexpr int B_BYTES = NT * 128;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = NT == 256 ? 4 : NT == 128 ? 6 : 8;
+  static constexpr int SUMS = NT <= 128 ? NT * 128 * 4 : 0;  // split tiles only (NT <= 128)
+  static constexpr int TMEM_COLS = NT < 32 ? 32 : NT;
+  static constexpr int PIPE = STAGES * STAGE_BYTES;
+  static constexpr int SMEM_BYTES = PIPE + 256;
+  static_assert(SUMS <= PIPE && SMEM_BYTES <= 232448, "rows GEMM stages");
+};
+
+__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+template <typename OUT>
+__device__ __forceinline__ void store_out(const S8Args& a, long m, int n, float v) {
+  if constexpr (sizeof(OUT) == 2) reinterpret_cast<bf16*>(a.C)[m * a.ldc + n] = __float2bfloat16(v);
+  else reinterpret_cast<float*>(a.C)[m * a.ldc + n] = v;
+}
+
+template <int NT, typename OUT>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_s8_rows(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const S8Args args,
+                 int splits) {
+  using C_ = RowsCfg<NT>;
+  extern __shared__ __align__(1024) uint8_t smem[];  // swizzle atoms start on 1024-byte boundaries
+  uint8_t* smem_a = smem;
+  uint8_t* smem_b = smem + C_::STAGES * C_::A_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C_::PIPE);
+  uint64_t* full_bar = bars;                    // [STAGES]
+  uint64_t* empty_bar = bars + C_::STAGES;      // [STAGES]
+  uint64_t* done_bar = bars + 2 * C_::STAGES;   // [1]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C_::STAGES + 1);
+
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  const int rank = splits > 1 ? (int)cluster_rank() : 0;
+  const int num_n = (args.N + 127) / 128;
+  const int tile = blockIdx.x / splits;
+  const int n0 = (tile % num_n) * 128;
+  const int m0 = (tile / num_n) * NT;
+  const int all_kb = (args.K + 127) / 128;
+  const int kb0 = (int)((long)all_kb * rank / splits), kb1 = (int)((long)all_kb * (rank + 1) / splits);
+  int* err = args.err;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C_::STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(done_bar, 1);
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C_::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  bool have = false;  // epilogue warps: this CTA's sums are in tensor memory
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued[C_::STAGES] = {};
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1, err, 71)) break;
+        mbar_arrive_expect_tx(&full_bar[stage], C_::STAGE_BYTES);
+        tma_load_2d(smem_a + stage * C_::A_BYTES, &tmW, &full_bar[stage], kb * 128, n0);
+        tma_load_2d(smem_b + stage * C_::B_BYTES, &tmX, &full_bar[stage], kb * 128, m0);
+        issued[stage]++;
+        if (++stage == C_::STAGES) { stage = 0; phase ^= 1; }
+      }
+      // every copy this thread issued has landed before the CTA can exit
+      for (int s = 0; s < C_::STAGES; ++s)
+        if (issued[s] > 0) mbar_wait_drain(&full_bar[s], (uint32_t)((issued[s] - 1) & 1));
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc_s8(128, NT);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&full_bar[stage], phase, err, 72)) break;
+        tc_fence_after();
+        const uint32_t sa = smem_u32(smem_a + stage * C_::A_BYTES);
+        const uint32_t sb = smem_u32(smem_b + stage * C_::B_BYTES);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          mma_s8(tmem_base, make_sdesc(sa + r * 32, 16, 1024, kLayoutSw128),
+                 make_sdesc(sb + r * 32, 16, 1024, kLayoutSw128), idesc, (kb > kb0 || r > 0) ? 1u : 0u);
+        mma_commit(&empty_bar[stage]);
+        if (++stage == C_::STAGES) { stage = 0; phase ^= 1; }
+      }
+      // arrives once every MMA issued above has completed
+      mma_commit(done_bar);
+      mbar_wait_drain(done_bar, 0);
+    }
+  } else {
+    have = mbar_wait(done_bar, 0, err, 73);
+    tc_fence_after();
+    const int quarter = warp & 3;
+    const int ch = quarter * 32 + lane, n = n0 + ch;
+    const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    constexpr int W = NT < 32 ? NT : 32;  // tokens a step
+    if (splits == 1) {
+      const float sb = n < args.N ? args.sb[n] : 0.f, bias = n < args.N ? bias_at(args, n) : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < NT && have; c += W) {
+        if (m0 + c >= args.M) break;
+        uint32_t v[W];
+        if constexpr (W == 32) tmem_ld32(tbase + c, v);
+        else tmem_ld16(tbase + c, v);
+        tmem_wait_ld();
+        if (n < args.N) {
+#pragma unroll
+          for (int j = 0; j < W; ++j) {
+            const int m = m0 + c + j;
+            if (m < args.M) store_out<OUT>(args, m, n, fmaf((float)(int)v[j] * args.sa[m], sb, bias));
+          }
+        }
+      }
+    } else {
+      // the pipeline's buffers are free: every copy into them was consumed by an MMA that is done
+      int* sums = reinterpret_cast<int*>(smem);
+#pragma unroll 1
+      for (int c = 0; c < NT && have; c += W) {
+        uint32_t v[W];
+        if constexpr (W == 32) tmem_ld32(tbase + c, v);
+        else tmem_ld16(tbase + c, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < W; ++j) sums[(c + j) * 128 + ch] = (int)v[j];
+      }
+    }
+  }
+
+  tc_fence_before();
+  if (splits > 1) {
+    cluster_sync_all();  // every rank's sums are written
+    if (warp >= 2 && have) {
+      const int ch = (warp & 3) * 32 + lane, n = n0 + ch;
+      const int per = NT / splits, t0 = rank * per;
+      if (n < args.N) {
+        const float sb = args.sb[n], bias = bias_at(args, n);
+        const uint32_t mine = smem_u32(smem) + (uint32_t)ch * 4;
+        for (int j = t0; j < t0 + per; ++j) {
+          const int m = m0 + j;
+          if (m >= args.M) break;
+          int sum = 0;
+          for (int r = 0; r < splits; ++r) sum += ld_cluster_s32(peer_addr(mine + (uint32_t)j * 512, (uint32_t)r));
+          store_out<OUT>(args, m, n, fmaf((float)sum * args.sa[m], sb, bias));
+        }
+      }
+    }
+    cluster_sync_all();  // no rank's memory goes away while another reads it
+  } else {
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C_::TMEM_COLS);
+  }
+}
+
 // CUDA-core kernel for operands TMA cannot address (rows that do not start on
 // 16-byte boundaries) and for K = 0.
 __global__ void __launch_bounds__(256) gemm_s8_simt(const S8Args a) {
@@ -74,6 +568,135 @@ __global__ void __launch_bounds__(256) gemm_s8_simt(const S8Args a) {
     const float v = (float)acc[i] * a.sa[m] * sb + bias;
     if (a.c_f32) reinterpret_cast<float*>(a.C)[(long)m * a.ldc + n] = v;
     else reinterpret_cast<bf16*>(a.C)[(long)m * a.ldc + n] = __float2bfloat16(v);
+  }
+}
+
+// 2-D map over a row-major [rows, cols] matrix with row stride `ld_bytes`; box =
+// 128 bytes x box_rows, 128-byte swizzle.
+CUtensorMap make_map(const void* base, CUtensorMapDataType type, int esize, long rows, long cols, long ld_bytes,
+                     int box_rows) {
+  CUtensorMap m;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld_bytes};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / esize), (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = get_encode_fn()(&m, type, 2, const_cast<void*>(base), dims, strides, box, estr,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "harp gemm_s8: cuTensorMapEncodeTiled failed (", std::to_string((int)r), ")");
+  return m;
+}
+CUtensorMap make_map_s8(const int8_t* base, long rows, long cols, long ld, int box_rows) {
+  return make_map(base, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, cols, ld, box_rows);
+}
+
+template <int BN, typename OUT>
+void launch_pair(const S8Args& a, bool c_tma, cudaStream_t stream) {
+  using C_ = PairCfg<BN>;
+  auto kern = gemm_s8_pair<BN, OUT>;
+  static int max_clusters = 0;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C_::SMEM_BYTES;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (max_clusters == 0) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM_BYTES));
+    cfg.gridDim = dim3(2 * (num_sms() / 2));
+    int n = 0;
+    C10_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+    max_clusters = std::max(1, n);
+  }
+  const CUtensorMap ta = make_map_s8(a.A, a.M, a.K, a.lda, 128), tb = make_map_s8(a.B, a.N, a.K, a.ldb, BN / 2);
+  CUtensorMap tc = ta;
+  if (c_tma)
+    tc = make_map(a.C, sizeof(OUT) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                  sizeof(OUT), a.M, a.N, a.ldc * (long)sizeof(OUT), 32);
+  const long tiles = (long)((a.M + 255) / 256) * ((a.N + BN - 1) / BN);
+  TORCH_CHECK(tiles <= 0x3FFFFFFF, "harp gemm_s8: too many tiles");
+  cfg.gridDim = dim3(2 * (unsigned)std::min<long>(tiles, max_clusters));
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, tc, a, c_tma ? 1 : 0));
+  count_launch();
+}
+
+template <int NT, typename OUT>
+void launch_rows(const S8Args& a, int splits, cudaStream_t stream) {
+  using C_ = RowsCfg<NT>;
+  auto kern = gemm_s8_rows<NT, OUT>;
+  static bool configured = false;
+  if (!configured) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM_BYTES));
+    configured = true;
+  }
+  const CUtensorMap tw = make_map_s8(a.B, a.N, a.K, a.ldb, 128), tx = make_map_s8(a.A, a.M, a.K, a.lda, NT);
+  const long ctas = (long)((a.N + 127) / 128) * ((a.M + NT - 1) / NT) * splits;
+  TORCH_CHECK(ctas <= 0x7FFFFFFF, "harp gemm_s8: too many tiles");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C_::SMEM_BYTES;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tw, tx, a, splits));
+  count_launch();
+}
+
+// Pair tile width: the one of 256 / 192 / 128 that wastes the least work in the
+// last column band and the last wave of clusters.
+int pick_bn(const S8Args& a) {
+  const int pairs = num_sms() / 2;
+  auto cost = [&](int bn) {
+    const long tiles = (long)((a.M + 255) / 256) * ((a.N + bn - 1) / bn);
+    return (double)((tiles + pairs - 1) / pairs) * bn / (bn == 256 ? 1.0 : (bn == 192 ? 0.87 : 0.67));
+  };
+  int best = 256;
+  for (int bn : {192, 128})
+    if (cost(bn) < cost(best) * 0.97) best = bn;
+  return best;
+}
+
+// Tokens a CTA and K splits of the rows kernel: as many CTAs as the GPU has SMs.
+void pick_rows(const S8Args& a, int& nt, int& splits) {
+  const int sms = num_sms();
+  const long chans = (a.N + 127) / 128;
+  const int kb = (a.K + 127) / 128;
+  nt = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+  while (nt < 256 && nt >= 128 && chans * ((a.M + nt - 1) / nt) > sms) nt *= 2;
+  splits = 1;
+  while (nt <= 128 && splits < 8 && 2 * splits <= kb && chans * ((a.M + nt - 1) / nt) * splits * 2 <= sms + sms / 8)
+    splits *= 2;
+}
+
+template <typename OUT>
+void dispatch(const S8Args& a, bool c_tma, cudaStream_t stream) {
+  if (a.M >= 512 && a.N >= 256) {
+    switch (pick_bn(a)) {
+      case 256: launch_pair<256, OUT>(a, c_tma, stream); break;
+      case 192: launch_pair<192, OUT>(a, c_tma, stream); break;
+      default: launch_pair<128, OUT>(a, c_tma, stream); break;
+    }
+    return;
+  }
+  int nt, splits;
+  pick_rows(a, nt, splits);
+  switch (nt) {
+    case 16: launch_rows<16, OUT>(a, splits, stream); break;
+    case 32: launch_rows<32, OUT>(a, splits, stream); break;
+    case 64: launch_rows<64, OUT>(a, splits, stream); break;
+    case 128: launch_rows<128, OUT>(a, splits, stream); break;
+    default: launch_rows<256, OUT>(a, splits, stream); break;
   }
 }
 
@@ -125,6 +748,20 @@ void gemm_s8(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, con
   a.ldc = C.stride(0);
   a.c_f32 = C.scalar_type() == at::kFloat;
   a.err = err.data_ptr<int>();
+  auto rows16 = [](const at::Tensor& t) {
+    return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 &&
+           (t.size(0) <= 1 || (t.stride(0) * t.element_size()) % 16 == 0);
+  };
+  // TMA: 16-byte aligned rows whose stride covers them (a stride of 0 or an overlap is left to the CUDA cores)
+  if (K > 0 && rows16(A) && rows16(B) && (M == 1 || a.lda >= K) && (N == 1 || a.ldb >= K)) {
+    const long pad = (K + 15) / 16 * 16;
+    if (M == 1) a.lda = pad;
+    if (N == 1) a.ldb = pad;
+    const bool c_tma = rows16(C) && (M == 1 || a.ldc >= N) && M > 1;
+    if (a.c_f32) dispatch<float>(a, c_tma, stream);
+    else dispatch<bf16>(a, c_tma, stream);
+    return;
+  }
   dim3 grid((unsigned)((N + 31) / 32), (unsigned)((M + 31) / 32));
   TORCH_CHECK(grid.y <= 65535, "harp gemm_s8: too many rows for the CUDA-core path");
   gemm_s8_simt<<<grid, 256, 0, stream>>>(a);

@@ -17,6 +17,7 @@
 //   warps 2..5  epilogue: tcgen05.ld of the accumulator (32 lanes per warp)
 // Two TMEM accumulators let the epilogue of tile i overlap the MMAs of tile i+1.
 #include "common.cuh"
+#include "gemm_common.cuh"
 #include "gemm_sm100.h"
 
 #include <ATen/cuda/CUDAContext.h>
@@ -45,7 +46,6 @@ struct WeightGate {
 std::mutex g_gate_mu;
 WeightGate g_gate;
 constexpr int kThreads = 192;
-constexpr int kGroupM = 8;
 
 struct GemmArgs {
   int M, N, K;
@@ -103,24 +103,6 @@ struct Cfg {
   static constexpr int TMEM_COLS = (2 * BN <= 256) ? 256 : 512;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/;
 };
-
-__device__ __forceinline__ void tile_coords(int t, int num_m, int num_n, int& mt, int& nt) {
-  const int group = kGroupM * num_n;
-  const int g = t / group;
-  const int first_m = g * kGroupM;
-  const int gm = min(num_m - first_m, kGroupM);
-  const int r = t % group;
-  mt = first_m + r % gm;
-  nt = r / gm;
-}
-
-__device__ __forceinline__ bool mbar_wait_drain(uint64_t* bar, uint32_t parity) {
-  const unsigned long long t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, parity)) {
-    if (globaltimer_ns() - t0 > 1000000000ull) return false;
-  }
-  return true;
-}
 
 template <int BN>
 __device__ __forceinline__ void epilogue_chunk(const GemmArgs& a, int m, int n, const uint32_t (&v)[32]) {
@@ -396,29 +378,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Every wait is bounded; errors fall through to the end, where both CTAs meet
 // at the cluster barrier before the paired TMEM is released.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t peer_addr(uint32_t local, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int c0,
-                                                 int c1) {
-  HARP_CHECK_TMA_X(c0, 204);
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
-      "[%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(c0), "r"(c1)
-      : "memory");
-}
 __device__ __forceinline__ void mma_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                             uint32_t accumulate) {
   HARP_CHECK_TMEM(d_tmem, (int)(((idesc >> 17) & 0x3Fu) << 3), 214);
@@ -426,24 +385,6 @@ __device__ __forceinline__ void mma_ss_pair(uint32_t d_tmem, uint64_t a_desc, ui
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate));
-}
-// arrive on the barrier at this shared::cluster address once the pair's MMAs issued so far are done
-__device__ __forceinline__ void mma_commit_pair(uint32_t bar_cluster) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_cluster)
-               : "memory");
-}
-__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, int ncols) {
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)),
-               "r"(ncols));
-}
-__device__ __forceinline__ void tmem_relinquish_pair() {
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
-}
-__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, int ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols));
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 
 // Each pipeline stage holds a K depth of 128 (two 128-byte swizzle atoms per
