@@ -20,6 +20,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -42,6 +43,7 @@ struct S8Args {
   void* C;
   long ldc;
   int c_f32;
+  int c_vec4;  // four neighbouring values of any row of C can be stored at once
   int* err;
 };
 
@@ -77,6 +79,14 @@ __device__ __forceinline__ void mma_s8_pair(uint32_t d_tmem, uint64_t a_desc, ui
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// arrive on the barrier at this offset in both CTAs of the pair once the MMAs issued so far are done
+__device__ __forceinline__ void mma_commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
       : "memory");
 }
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
@@ -122,7 +132,31 @@ struct PairCfg {
   static_assert(STAGES >= 3 && STAGES <= 8 && SMEM_BYTES <= 232448, "pair GEMM stages");
 };
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// Arrive on another CTA's barrier without ordering earlier stores: what the
+// barrier hands over is tensor memory, which the tcgen05 fences order.  (With
+// release.cluster the arrive waits for the stores of the epilogue: 1700 clocks a
+// tile, and the accumulator is free that much later.)
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
 __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// Order of the pair kernel's tiles: the whole ones first, those of a last column
+// band narrower than the tile at the end, where they even out the last wave.
+__device__ __forceinline__ void pair_tile(int t, int num_m, int num_n, bool narrow, int& mt, int& nt) {
+  const int whole = narrow ? num_n - 1 : num_n;
+  if (t < num_m * whole) {
+    tile_coords(t, num_m, whole, mt, nt);
+  } else {
+    mt = t - num_m * whole;
+    nt = whole;
+  }
+}
 
 template <int BN, typename OUT>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -189,14 +223,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t fb0 = peer_addr(smem_u32(&full_bar[0]), 0);  // the leader's barriers
       for (int t = pair; t < num_tiles && ok; t += npairs) {
         int mt, nt;
-        tile_coords(t, num_m, num_n, mt, nt);
-        const int m0 = mt * 256 + (int)rank * 128, n0 = nt * BN + (int)rank * (BN / 2);
+        pair_tile(t, num_m, num_n, args.N % BN != 0, mt, nt);
+        // a narrow tile multiplies only the columns it has, half of them from each CTA
+        const int half = min(BN / 2, ((args.N - nt * BN + 31) / 32) * 16);
+        const int m0 = mt * 256 + (int)rank * 128, n0 = nt * BN + (int)rank * half;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, err, 61)) { ok = false; break; }
           const uint32_t fb = fb0 + stage * 8;
-          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * C_::STAGE_BYTES);
-#pragma unroll
-          for (int h = 0; h < kStageK / 128; ++h) {
+          const int atoms = min(kStageK / 128, (args.K - kb * kStageK + 127) / 128);  // the last stage may be half
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * C_::STAGE_BYTES / (kStageK / 128) * atoms);
+          for (int h = 0; h < atoms; ++h) {
             const int k0 = kb * kStageK + h * 128;
             tma_load_2d_pair(smem_a + stage * C_::A_BYTES + h * C_::A_ATOM, &tmA, fb, k0, m0);
             tma_load_2d_pair(smem_b + stage * C_::B_BYTES + h * C_::B_ATOM, &tmB, fb, k0, n0);
@@ -212,8 +248,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (leader CTA) ----------------
-    if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc = make_idesc_s8(256, BN);
+    // The whole warp keeps the loop's state, so that it stays in uniform registers; one lane issues.
+    if (rank == 0) {
+      const bool issue = elect_one();
+      const uint64_t a0 = make_sdesc(smem_u32(smem_a), 16, 1024, kLayoutSw128);
+      const uint64_t b0 = make_sdesc(smem_u32(smem_b), 16, 1024, kLayoutSw128);
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
@@ -224,31 +263,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1, err, 62)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
+        int mt, nt;
+        pair_tile(t, num_m, num_n, args.N % BN != 0, mt, nt);
+        const uint32_t idesc = make_idesc_s8(256, 2 * min(BN / 2, ((args.N - nt * BN + 31) / 32) * 16));
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&full_bar[stage], phase, err, 63)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem_a + stage * C_::A_BYTES);
-          const uint32_t sb = smem_u32(smem_b + stage * C_::B_BYTES);
+          const uint64_t ad = a0 + (uint64_t)(stage * (C_::A_BYTES >> 4));
+          const uint64_t bd = b0 + (uint64_t)(stage * (C_::B_BYTES >> 4));
+          const bool second = kb * kStageK + 128 < args.K;
+          if (issue) {
 #pragma unroll
-          for (int kk = 0; kk < kStageK / 32; ++kk) {
-            const int h = kk / 4, r = kk % 4;
-            const uint64_t adesc = make_sdesc(sa + h * C_::A_ATOM + r * 32, 16, 1024, kLayoutSw128);
-            const uint64_t bdesc = make_sdesc(sb + h * C_::B_ATOM + r * 32, 16, 1024, kLayoutSw128);
-            mma_s8_pair(d_tmem, adesc, bdesc, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+            for (int r = 0; r < 4; ++r)
+              mma_s8_pair(d_tmem, ad + r * 2, bd + r * 2, idesc, (kb > 0 || r > 0) ? 1u : 0u);
+            if (second) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                mma_s8_pair(d_tmem, ad + (C_::A_ATOM >> 4) + r * 2, bd + (C_::B_ATOM >> 4) + r * 2, idesc, 1u);
+            }
+            mma_commit_both(&empty_bar[stage]);
           }
-          const uint32_t eb = smem_u32(&empty_bar[stage]);
-          mma_commit_pair(eb);
-          mma_commit_pair(peer_addr(eb, 1));
+          __syncwarp();
           if (++stage == C_::STAGES) { stage = 0; phase ^= 1; }
         }
         if (!ok) break;
-        const uint32_t tf = smem_u32(&tfull_bar[acc]);
-        mma_commit_pair(tf);
-        mma_commit_pair(peer_addr(tf, 1));
+        if (issue) mma_commit_both(&tfull_bar[acc]);
+        __syncwarp();
       }
-      const uint32_t db = smem_u32(drain_bar);
-      mma_commit_pair(db);
-      mma_commit_pair(peer_addr(db, 1));
+      if (issue) mma_commit_both(drain_bar);
+      __syncwarp();
     }
     // both CTAs: the pair's MMAs are done before the paired TMEM goes away
     if (lane == 0) mbar_wait_drain(drain_bar, 0);
@@ -260,21 +303,41 @@ __global__ void __launch_bounds__(kThreads, 1)
     int local = 0, nbuf = 0;
     bool ok = true;  // after a failed wait the warp only keeps meeting the others at the barriers
     const uint32_t te_leader[2] = {peer_addr(smem_u32(&tempty_bar[0]), 0), peer_addr(smem_u32(&tempty_bar[1]), 0)};
+    // a tile's scales and bias are fetched while the one before it is being stored
+    constexpr int VPT = (BN + 127) / 128;
+    float sa_next = 0.f, sb_next[VPT], bias_next[VPT];
+    auto fetch = [&](int t) {
+      int mt, nt;
+      pair_tile(t, num_m, num_n, args.N % BN != 0, mt, nt);
+      const int m = mt * 256 + (int)rank * 128 + quarter * 32 + lane;
+      sa_next = m < args.M ? __ldg(args.sa + m) : 0.f;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int j = et + i * 128, n = nt * BN + j;
+        const bool in = j < BN && n < args.N;
+        sb_next[i] = in ? __ldg(args.sb + n) : 0.f;
+        bias_next[i] = in ? bias_at(args, n) : 0.f;
+      }
+    };
+    if (pair < num_tiles) fetch(pair);
     for (int t = pair; t < num_tiles; t += npairs, ++local) {
       int mt, nt;
-      tile_coords(t, num_m, num_n, mt, nt);
+      pair_tile(t, num_m, num_n, args.N % BN != 0, mt, nt);
       const int acc = local & 1;
       const uint32_t acc_phase = (local >> 1) & 1;
       const int mw = mt * 256 + (int)rank * 128 + quarter * 32;  // the warp's first row
-      const float sa = mw + lane < args.M ? args.sa[mw + lane] : 0.f;
-      // this tile's channel scales and bias, once every warp is done with the last tile's
-      if (local > 0) epilogue_barrier();
-      for (int j = et; j < BN; j += 128) {
-        const int n = nt * BN + j;
-        vecs[j] = n < args.N ? args.sb[n] : 0.f;
-        vecs[BN + j] = n < args.N ? bias_at(args, n) : 0.f;
+      const float sa = sa_next;
+      if (local > 0) epilogue_barrier();  // every warp is done with the last tile's
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int j = et + i * 128;
+        if (j < BN) {
+          vecs[j] = sb_next[i];
+          vecs[BN + j] = bias_next[i];
+        }
       }
       epilogue_barrier();
+      if (t + npairs < num_tiles) fetch(t + npairs);
       ok = ok && mbar_wait(&tfull_bar[acc], acc_phase, err, 64);
       if (!ok) continue;
       tc_fence_after();
@@ -296,7 +359,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j4 = 0; j4 < 8; ++j4) {
             const float4 s4 = *reinterpret_cast<const float4*>(vecs + c * CW + g * 32 + j4 * 4);
-            const float4 b4 = *reinterpret_cast<const float4*>(vecs + BN + c * CW + g * 32 + j4 * 4);
+            float4 b4 = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (args.bias != nullptr) b4 = *reinterpret_cast<const float4*>(vecs + BN + c * CW + g * 32 + j4 * 4);
             const float x0 = fmaf((float)(int)v[4 * j4 + 0] * sa, s4.x, b4.x);
             const float x1 = fmaf((float)(int)v[4 * j4 + 1] * sa, s4.y, b4.y);
             const float x2 = fmaf((float)(int)v[4 * j4 + 2] * sa, s4.z, b4.z);
@@ -339,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(te_leader[acc]);
+      if (lane == 0) mbar_arrive_remote(te_leader[acc]);
     }
     if (lane == 0) bulk_wait_read<0>();  // the staging buffers outlive the stores that read them
   }
@@ -356,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Few tokens or few channels.  A CTA multiplies 128 channels (the MMA's M) by NT
 // tokens (its N) over its share of K; a cluster of `splits` CTAs along x covers
 // K.  Each CTA of a split tile leaves its integer sums in its shared memory, the
-// cluster meets, and rank r adds and stores tokens r*NT/splits onwards, read from
+// cluster meets, and rank r adds and stores the r-th part of the tokens, read from
 // every rank's memory: one launch, no workspace, and the same sum in any order.
 // ---------------------------------------------------------------------------
 template <int NT>
@@ -365,22 +429,37 @@ struct RowsCfg {
   static constexpr int B_BYTES = NT * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGES = NT == 256 ? 4 : NT == 128 ? 6 : 8;
-  static constexpr int SUMS = NT <= 128 ? NT * 128 * 4 : 0;  // split tiles only (NT <= 128)
+  static constexpr int SUMS = NT * 128 * 4;  // the tile's integer sums [NT][128], over the pipeline's buffers
   static constexpr int TMEM_COLS = NT < 32 ? 32 : NT;
   static constexpr int PIPE = STAGES * STAGE_BYTES;
-  static constexpr int SMEM_BYTES = PIPE + 256;
+  static constexpr int SMEM_BYTES = PIPE + NT * 4 + 256;
   static_assert(SUMS <= PIPE && SMEM_BYTES <= 232448, "rows GEMM stages");
 };
 
-__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ int4 ld_cluster_v4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
+// Four neighbouring channels of token m.
 template <typename OUT>
-__device__ __forceinline__ void store_out(const S8Args& a, long m, int n, float v) {
-  if constexpr (sizeof(OUT) == 2) reinterpret_cast<bf16*>(a.C)[m * a.ldc + n] = __float2bfloat16(v);
-  else reinterpret_cast<float*>(a.C)[m * a.ldc + n] = v;
+__device__ __forceinline__ void store_out4(const S8Args& a, long m, int n, float v0, float v1, float v2, float v3) {
+  OUT* c = reinterpret_cast<OUT*>(a.C) + m * a.ldc + n;
+  if (a.c_vec4 && n + 4 <= a.N) {
+    if constexpr (sizeof(OUT) == 2) *reinterpret_cast<uint2*>(c) = make_uint2(pack_bf16x2(v0, v1), pack_bf16x2(v2, v3));
+    else *reinterpret_cast<float4*>(c) = make_float4(v0, v1, v2, v3);
+    return;
+  }
+  const float v[4] = {v0, v1, v2, v3};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (n + i >= a.N) continue;
+    if constexpr (sizeof(OUT) == 2) c[i] = __float2bfloat16(v[i]);
+    else c[i] = v[i];
+  }
 }
 
 template <int NT, typename OUT>
@@ -391,7 +470,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem[];  // swizzle atoms start on 1024-byte boundaries
   uint8_t* smem_a = smem;
   uint8_t* smem_b = smem + C_::STAGES * C_::A_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C_::PIPE);
+  float* tok_scale = reinterpret_cast<float*>(smem + C_::PIPE);  // [NT]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C_::PIPE + NT * 4);
   uint64_t* full_bar = bars;                    // [STAGES]
   uint64_t* empty_bar = bars + C_::STAGES;      // [STAGES]
   uint64_t* done_bar = bars + 2 * C_::STAGES;   // [1]
@@ -448,87 +528,81 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (issued[s] > 0) mbar_wait_drain(&full_bar[s], (uint32_t)((issued[s] - 1) & 1));
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = make_idesc_s8(128, NT);
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&full_bar[stage], phase, err, 72)) break;
-        tc_fence_after();
-        const uint32_t sa = smem_u32(smem_a + stage * C_::A_BYTES);
-        const uint32_t sb = smem_u32(smem_b + stage * C_::B_BYTES);
+    constexpr uint32_t idesc = make_idesc_s8(128, NT);
+    const bool issue = elect_one();
+    const uint64_t a0 = make_sdesc(smem_u32(smem_a), 16, 1024, kLayoutSw128);
+    const uint64_t b0 = make_sdesc(smem_u32(smem_b), 16, 1024, kLayoutSw128);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait(&full_bar[stage], phase, err, 72)) break;
+      tc_fence_after();
+      if (issue) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          mma_s8(tmem_base, make_sdesc(sa + r * 32, 16, 1024, kLayoutSw128),
-                 make_sdesc(sb + r * 32, 16, 1024, kLayoutSw128), idesc, (kb > kb0 || r > 0) ? 1u : 0u);
+          mma_s8(tmem_base, a0 + (uint64_t)(stage * (C_::A_BYTES >> 4) + r * 2),
+                 b0 + (uint64_t)(stage * (C_::B_BYTES >> 4) + r * 2), idesc, (kb > kb0 || r > 0) ? 1u : 0u);
         mma_commit(&empty_bar[stage]);
-        if (++stage == C_::STAGES) { stage = 0; phase ^= 1; }
       }
-      // arrives once every MMA issued above has completed
-      mma_commit(done_bar);
-      mbar_wait_drain(done_bar, 0);
+      __syncwarp();
+      if (++stage == C_::STAGES) { stage = 0; phase ^= 1; }
     }
+    // arrives once every MMA issued above has completed
+    if (issue) mma_commit(done_bar);
+    __syncwarp();
+    if (lane == 0) mbar_wait_drain(done_bar, 0);
   } else {
+    const int quarter = warp & 3;
+    const int ch = quarter * 32 + lane;
+    for (int j = threadIdx.x - 64; j < NT; j += 128) tok_scale[j] = m0 + j < args.M ? args.sa[m0 + j] : 0.f;
     have = mbar_wait(done_bar, 0, err, 73);
     tc_fence_after();
-    const int quarter = warp & 3;
-    const int ch = quarter * 32 + lane, n = n0 + ch;
     const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16);
     constexpr int W = NT < 32 ? NT : 32;  // tokens a step
-    if (splits == 1) {
-      const float sb = n < args.N ? args.sb[n] : 0.f, bias = n < args.N ? bias_at(args, n) : 0.f;
+    // the pipeline's buffers are free: every copy into them was consumed by an MMA that is done
+    int* sums = reinterpret_cast<int*>(smem);
 #pragma unroll 1
-      for (int c = 0; c < NT && have; c += W) {
-        if (m0 + c >= args.M) break;
-        uint32_t v[W];
-        if constexpr (W == 32) tmem_ld32(tbase + c, v);
-        else tmem_ld16(tbase + c, v);
-        tmem_wait_ld();
-        if (n < args.N) {
+    for (int c = 0; c < NT && have && m0 + c < args.M; c += W) {
+      uint32_t v[W];
+      if constexpr (W == 32) tmem_ld32(tbase + c, v);
+      else tmem_ld16(tbase + c, v);
+      tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < W; ++j) {
-            const int m = m0 + c + j;
-            if (m < args.M) store_out<OUT>(args, m, n, fmaf((float)(int)v[j] * args.sa[m], sb, bias));
-          }
-        }
-      }
-    } else {
-      // the pipeline's buffers are free: every copy into them was consumed by an MMA that is done
-      int* sums = reinterpret_cast<int*>(smem);
-#pragma unroll 1
-      for (int c = 0; c < NT && have; c += W) {
-        uint32_t v[W];
-        if constexpr (W == 32) tmem_ld32(tbase + c, v);
-        else tmem_ld16(tbase + c, v);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < W; ++j) sums[(c + j) * 128 + ch] = (int)v[j];
-      }
+      for (int j = 0; j < W; ++j) sums[(c + j) * 128 + ch] = (int)v[j];
     }
   }
 
   tc_fence_before();
-  if (splits > 1) {
-    cluster_sync_all();  // every rank's sums are written
-    if (warp >= 2 && have) {
-      const int ch = (warp & 3) * 32 + lane, n = n0 + ch;
-      const int per = NT / splits, t0 = rank * per;
-      if (n < args.N) {
-        const float sb = args.sb[n], bias = bias_at(args, n);
-        const uint32_t mine = smem_u32(smem) + (uint32_t)ch * 4;
-        for (int j = t0; j < t0 + per; ++j) {
-          const int m = m0 + j;
-          if (m >= args.M) break;
-          int sum = 0;
-          for (int r = 0; r < splits; ++r) sum += ld_cluster_s32(peer_addr(mine + (uint32_t)j * 512, (uint32_t)r));
-          store_out<OUT>(args, m, n, fmaf((float)sum * args.sa[m], sb, bias));
-        }
-      }
+  if (splits > 1) cluster_sync_all();  // every rank's sums are written
+  else __syncthreads();
+  if (warp >= 2 && have) {
+    // a warp takes every fourth token of this rank's share, a lane four channels of it
+    const int t0 = rank * NT / splits, t1 = (rank + 1) * NT / splits, n = n0 + lane * 4;
+    float sb[4], bias[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sb[i] = n + i < args.N ? args.sb[n + i] : 0.f;
+      bias[i] = n + i < args.N ? bias_at(args, n + i) : 0.f;
     }
-    cluster_sync_all();  // no rank's memory goes away while another reads it
-  } else {
-    __syncthreads();
+    const uint32_t mine = smem_u32(smem) + (uint32_t)lane * 16;
+#pragma unroll 4
+    for (int j = t0 + warp - 2; j < t1; j += 4) {
+      if (m0 + j >= args.M) break;
+      int4 sum = make_int4(0, 0, 0, 0);
+      if (splits > 1) {
+        for (int r = 0; r < splits; ++r) {
+          const int4 v = ld_cluster_v4(peer_addr(mine + (uint32_t)j * 512, (uint32_t)r));
+          sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+        }
+      } else {
+        sum = *reinterpret_cast<const int4*>(smem + j * 512 + lane * 16);
+      }
+      const float sa = tok_scale[j];
+      store_out4<OUT>(args, m0 + j, n, fmaf((float)sum.x * sa, sb[0], bias[0]), fmaf((float)sum.y * sa, sb[1], bias[1]),
+                      fmaf((float)sum.z * sa, sb[2], bias[2]), fmaf((float)sum.w * sa, sb[3], bias[3]));
+    }
   }
+  if (splits > 1) cluster_sync_all();  // no rank's memory goes away while another reads it
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, C_::TMEM_COLS);
@@ -653,50 +727,91 @@ void launch_rows(const S8Args& a, int splits, cudaStream_t stream) {
   count_launch();
 }
 
-// Pair tile width: the one of 256 / 192 / 128 that wastes the least work in the
-// last column band and the last wave of clusters.
-int pick_bn(const S8Args& a) {
-  const int pairs = num_sms() / 2;
-  auto cost = [&](int bn) {
-    const long tiles = (long)((a.M + 255) / 256) * ((a.N + bn - 1) / bn);
-    return (double)((tiles + pairs - 1) / pairs) * bn / (bn == 256 ? 1.0 : (bn == 192 ? 0.87 : 0.67));
-  };
-  int best = 256;
-  for (int bn : {192, 128})
-    if (cost(bn) < cost(best) * 0.97) best = bn;
-  return best;
+// CTAs of the rows kernel that run at once in clusters of `splits` (larger clusters
+// leave SMs of a GPC over).
+long cluster_slots(int splits) {
+  static std::atomic<long> slots[9];
+  if (splits == 1) return num_sms();
+  long n = slots[splits].load(std::memory_order_relaxed);
+  if (n == 0) {
+    using C_ = RowsCfg<16>;
+    auto kern = gemm_s8_rows<16, bf16>;
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM_BYTES));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(num_sms() / splits * splits));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C_::SMEM_BYTES;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    C10_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg));
+    n = std::max(1, clusters * splits);
+    slots[splits].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
-
-// Tokens a CTA and K splits of the rows kernel: as many CTAs as the GPU has SMs.
-void pick_rows(const S8Args& a, int& nt, int& splits) {
+// The kernel and its tile by estimated time.  The constants are microseconds
+// measured on a B200: an SM takes in 135 KB a microsecond, all of them 14 MB; a pair
+// multiplies 256 x BN x 128 in 0.0014 BN; the epilogues take time by the columns a
+// CTA stores; a second wave of single-tile CTAs starts only when the first is done.
+// Of 44 shapes (M = 1 .. 17408, N = 24 .. 9216, K = 32 .. 6144) timed with every tile
+// and split, the choice was within 8 % of the fastest at 41 and within 20 % at all:
+// 4 x 1152 x 4608 takes 5.7 us with 8 splits and 10.8 with one; 1088 x 9216 x 1152 takes
+// 17.5 on CTA pairs and 30 in the rows kernel; 64 x 3456 x 1152 5.9 there and 6.7 on pairs.
+struct Plan {
+  int pair_bn;  // 256 / 192 / 128, or 0: the rows kernel with
+  int nt, splits;
+};
+Plan pick(const S8Args& a) {
   const int sms = num_sms();
   const long chans = (a.N + 127) / 128;
   const int kb = (a.K + 127) / 128;
-  nt = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
-  while (nt < 256 && nt >= 128 && chans * ((a.M + nt - 1) / nt) > sms) nt *= 2;
-  splits = 1;
-  while (nt <= 128 && splits < 8 && 2 * splits <= kb && chans * ((a.M + nt - 1) / nt) * splits * 2 <= sms + sms / 8)
-    splits *= 2;
+  auto load = [&](long ctas, double bytes) {
+    return bytes * std::max(1.0 / 135e3, (double)std::min<long>(ctas, sms) / 14e6);
+  };
+  Plan best = {0, 16, 1};
+  double best_t = 1e30;
+  for (int nt : {16, 32, 64, 128, 256}) {
+    const long tiles = chans * ((a.M + nt - 1) / nt);
+    for (int sp = 1; sp <= 8 && sp <= kb; ++sp) {
+      const long slots = cluster_slots(sp);
+      const long waves = (tiles * sp + slots - 1) / slots;
+      const double one = 4.0 + (kb + sp - 1) / sp * load(tiles * sp, 16384 + 128 * nt) + 0.016 * nt +
+                         (sp == 1 ? 0.0 : sp == 2 ? 1.0 : 0.5);
+      const double t = 2.0 + waves * (one - 2.0);
+      if (t < best_t) { best_t = t; best = {0, nt, sp}; }
+    }
+  }
+  for (int bn : {128, 192, 256}) {
+    const long tiles = (long)((a.M + 255) / 256) * ((a.N + bn - 1) / bn);
+    const long waves = (tiles + sms / 2 - 1) / (sms / 2);
+    const double stage = load(2 * tiles, (128 + bn / 2) * 128);
+    const double t = 3.5 + 0.0125 * bn + kb * stage + (waves - 1) * (kb * std::max(stage, 0.0014 * bn) + 0.5);
+    if (t < best_t) { best_t = t; best = {bn, 0, 0}; }
+  }
+  return best;
 }
 
 template <typename OUT>
 void dispatch(const S8Args& a, bool c_tma, cudaStream_t stream) {
-  if (a.M >= 512 && a.N >= 256) {
-    switch (pick_bn(a)) {
-      case 256: launch_pair<256, OUT>(a, c_tma, stream); break;
-      case 192: launch_pair<192, OUT>(a, c_tma, stream); break;
-      default: launch_pair<128, OUT>(a, c_tma, stream); break;
-    }
-    return;
+  const Plan p = pick(a);
+  switch (p.pair_bn) {
+    case 256: launch_pair<256, OUT>(a, c_tma, stream); return;
+    case 192: launch_pair<192, OUT>(a, c_tma, stream); return;
+    case 128: launch_pair<128, OUT>(a, c_tma, stream); return;
+    default: break;
   }
-  int nt, splits;
-  pick_rows(a, nt, splits);
-  switch (nt) {
-    case 16: launch_rows<16, OUT>(a, splits, stream); break;
-    case 32: launch_rows<32, OUT>(a, splits, stream); break;
-    case 64: launch_rows<64, OUT>(a, splits, stream); break;
-    case 128: launch_rows<128, OUT>(a, splits, stream); break;
-    default: launch_rows<256, OUT>(a, splits, stream); break;
+  switch (p.nt) {
+    case 16: launch_rows<16, OUT>(a, p.splits, stream); break;
+    case 32: launch_rows<32, OUT>(a, p.splits, stream); break;
+    case 64: launch_rows<64, OUT>(a, p.splits, stream); break;
+    case 128: launch_rows<128, OUT>(a, p.splits, stream); break;
+    default: launch_rows<256, OUT>(a, p.splits, stream); break;
   }
 }
 
@@ -708,8 +823,8 @@ void check_scales(const at::Tensor& s, const at::Tensor& rows, const char* name)
 
 }  // namespace
 
-void gemm_s8(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, const at::Tensor& sb,
-             const c10::optional<at::Tensor>& bias, at::Tensor& C, at::Tensor& err) {
+void gemm_s8_out(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, const at::Tensor& sb,
+                 const c10::optional<at::Tensor>& bias, at::Tensor C, at::Tensor err) {
   TORCH_CHECK(A.is_cuda() && B.is_cuda() && C.is_cuda() && err.is_cuda(), "harp gemm_s8: CUDA tensors required");
   TORCH_CHECK(A.device() == B.device() && A.device() == C.device() && A.device() == err.device(),
               "harp gemm_s8: operands on one device");
@@ -734,7 +849,7 @@ void gemm_s8(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, con
   if (M == 0 || N == 0) return;
   const at::cuda::CUDAGuard guard(A.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  S8Args a;
+  S8Args a = {};
   a.M = (int)M; a.N = (int)N; a.K = (int)K;
   a.A = reinterpret_cast<const int8_t*>(A.data_ptr());
   a.lda = A.stride(0);
@@ -758,6 +873,8 @@ void gemm_s8(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, con
     if (M == 1) a.lda = pad;
     if (N == 1) a.ldb = pad;
     const bool c_tma = rows16(C) && (M == 1 || a.ldc >= N) && M > 1;
+    const uintptr_t where = reinterpret_cast<uintptr_t>(a.C) | (M == 1 ? 0 : (uintptr_t)(a.ldc * C.element_size()));
+    a.c_vec4 = where % (4 * C.element_size()) == 0;
     if (a.c_f32) dispatch<float>(a, c_tma, stream);
     else dispatch<bf16>(a, c_tma, stream);
     return;
@@ -767,6 +884,14 @@ void gemm_s8(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, con
   gemm_s8_simt<<<grid, 256, 0, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   count_launch();
+}
+
+at::Tensor gemm_s8(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, const at::Tensor& sb,
+                   const c10::optional<at::Tensor>& bias, bool f32, at::Tensor err) {
+  TORCH_CHECK(A.is_cuda() && A.dim() == 2 && B.dim() == 2, "harp gemm_s8: 2-D CUDA operands");
+  at::Tensor C(at::detail::empty_cuda({A.size(0), B.size(0)}, f32 ? at::kFloat : at::kBFloat16, A.device(), c10::nullopt));
+  gemm_s8_out(A, sa, B, sb, bias, C, err);
+  return C;
 }
 
 }  // namespace harp

@@ -66,8 +66,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rmsnorm_mod_quant(
     const c10::optional<at::Tensor>& residual, const c10::optional<at::Tensor>& gate);
 at::Tensor dequant_rows(const at::Tensor& q, const at::Tensor& s, bool f32);
 // gemm_s8_sm100.cu
-void gemm_s8(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, const at::Tensor& sb,
-             const c10::optional<at::Tensor>& bias, at::Tensor& C, at::Tensor& err);
+at::Tensor gemm_s8(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, const at::Tensor& sb,
+                   const c10::optional<at::Tensor>& bias, bool f32, at::Tensor err);
+void gemm_s8_out(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, const at::Tensor& sb,
+                 const c10::optional<at::Tensor>& bias, at::Tensor C, at::Tensor err);
 
 namespace {
 
@@ -257,7 +259,8 @@ TORCH_LIBRARY(harp, m) {
   m.def("rmsnorm_mod_quant(Tensor x, Tensor? w, Tensor? scale, Tensor? shift, int rows_per_batch, float eps, "
         "Tensor? residual, Tensor? gate) -> (Tensor, Tensor, Tensor)");
   m.def("dequant_rows(Tensor q, Tensor s, bool f32) -> Tensor");
-  m.def("gemm_s8(Tensor A, Tensor sa, Tensor B, Tensor sb, Tensor? bias, Tensor(a!) C, Tensor(b!) err) -> ()");
+  m.def("gemm_s8(Tensor A, Tensor sa, Tensor B, Tensor sb, Tensor? bias, bool f32, Tensor(a!) err) -> Tensor");
+  m.def("gemm_s8_out(Tensor A, Tensor sa, Tensor B, Tensor sb, Tensor? bias, Tensor(a!) C, Tensor(b!) err) -> ()");
   m.def("launch_count() -> int");
   m.def("add_launch_count(int n) -> ()");
   m.def("reset_launch_count() -> ()");
@@ -291,6 +294,7 @@ TORCH_LIBRARY_IMPL(harp, CUDA, m) {
   m.impl("rmsnorm_mod_quant", &harp::rmsnorm_mod_quant);
   m.impl("dequant_rows", &harp::dequant_rows);
   m.impl("gemm_s8", &harp::gemm_s8);
+  m.impl("gemm_s8_out", &harp::gemm_s8_out);
 }
 
 TORCH_LIBRARY_IMPL(harp, CompositeExplicitAutograd, m) {

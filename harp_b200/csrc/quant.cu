@@ -23,6 +23,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -375,8 +376,8 @@ bool vec_ok(const at::Tensor& t) {
 // q [R, D] with rows on 16-byte boundaries (what TMA can address), s [R]
 std::tuple<at::Tensor, at::Tensor> new_rows8(const at::Tensor& x, int64_t R, int64_t D) {
   const int64_t ld = (D + 15) / 16 * 16;
-  auto q = at::empty({R, ld}, x.options().dtype(at::kChar));
-  auto s = at::empty({R}, x.options().dtype(at::kFloat));
+  at::Tensor q(at::detail::empty_cuda({R, ld}, at::kChar, x.device(), c10::nullopt));
+  at::Tensor s(at::detail::empty_cuda({R}, at::kFloat, x.device(), c10::nullopt));
   return {ld == D ? q : q.narrow(1, 0, D), s};
 }
 
@@ -462,7 +463,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rmsnorm_mod_quant(
                 op, ": residual must have x's shape, type and device and a unit inner stride");
     a.res = residual->data_ptr();
     a.ldr = residual->stride(0);
-    h = at::empty({R, D}, x.options());
+    h = at::Tensor(at::detail::empty_cuda({R, D}, x.scalar_type(), x.device(), c10::nullopt));
     a.h = h.data_ptr();
     a.ldh = D;
     vec = vec && vec_ok(*residual);
@@ -484,7 +485,7 @@ at::Tensor dequant_rows(const at::Tensor& q, const at::Tensor& s, bool f32) {
               "dequant_rows: s must be a dense fp32 vector with a scale for each row, on q's device");
   const at::cuda::CUDAGuard guard(q.device());
   const long R = q.size(0), D = q.size(1);
-  auto out = at::empty({R, D}, q.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+  at::Tensor out(at::detail::empty_cuda({R, D}, f32 ? at::kFloat : at::kBFloat16, q.device(), c10::nullopt));
   if (R == 0 || D == 0) return out;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const unsigned grid = (unsigned)std::min<long>(R, 1L << 20);

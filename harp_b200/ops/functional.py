@@ -493,11 +493,13 @@ def gemm_s8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
 
     The operands come from the quantisers above.  Their rows may have any stride; the
     tensor-core kernels take operands whose rows start on 16-byte boundaries."""
-    M, N = a.shape[0], b.shape[0]
-    if out is None:
-        out = torch.empty(M, N, device=a.device, dtype=out_dtype)
+    if out is None and out_dtype not in (torch.bfloat16, torch.float32):
+        raise RuntimeError(f"gemm_s8: bf16 or fp32 output, not {out_dtype}")
     if _cuda(a):
-        torch.ops.harp.gemm_s8(a, a_scale, b, b_scale, bias, out, errors.word(a.device))
+        if out is None:
+            return torch.ops.harp.gemm_s8(a, a_scale, b, b_scale, bias, out_dtype == torch.float32,
+                                          errors.word(a.device))
+        torch.ops.harp.gemm_s8_out(a, a_scale, b, b_scale, bias, out, errors.word(a.device))
         return out
     if a.dtype != torch.int8 or b.dtype != torch.int8 or a.shape[1] != b.shape[1]:
         raise RuntimeError("gemm_s8: int8 operands [M, K] and [N, K] are required")
@@ -507,6 +509,8 @@ def gemm_s8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
     acc = acc * a_scale[:, None] * b_scale[None, :]
     if bias is not None:
         acc = acc + bias.float()
+    if out is None:
+        return acc.to(out_dtype)
     out.copy_(acc.to(out.dtype))
     return out
 
