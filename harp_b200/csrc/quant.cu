@@ -27,6 +27,8 @@
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <mutex>
+
 namespace harp {
 
 namespace {
@@ -35,6 +37,7 @@ using bf16 = __nv_bfloat16;
 
 constexpr float kMinScale = 1.17549435e-38f;  // 2^-126
 constexpr int kMaxWarps = 16;
+constexpr size_t kVecSmem = 96 * 1024;  // of a sample's vectors in norm_sample_kernel
 
 enum QuantMode : int { kRows = 0, kSwiglu = 1, kNorm = 2, kNormRes = 3 };
 
@@ -64,27 +67,60 @@ __device__ __forceinline__ float to_f(bf16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void from_f(float v, float* p) { *p = v; }
 __device__ __forceinline__ void from_f(float v, bf16* p) { *p = __float2bfloat16(v); }
 
-// V consecutive values as fp32 (V = 8: 16-byte aligned).
+// V consecutive values as they are stored (V = 8: 16-byte aligned), and as fp32.
 template <int V, typename T>
-__device__ __forceinline__ void load_v(const T* p, float (&f)[V]) {
+struct Raw {
+  static constexpr int W = V * (int)sizeof(T) >= 16 ? V * (int)sizeof(T) / 16 : 1;
+  uint4 w[W];
+};
+template <typename T>
+struct Raw<1, T> {
+  T v;
+};
+template <int V, typename T>
+__device__ __forceinline__ Raw<V, T> load_raw(const T* p) {
+  Raw<V, T> r;
   if constexpr (V == 1) {
-    f[0] = to_f(*p);
-  } else if constexpr (sizeof(T) == 2) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f[2 * j] = __uint_as_float(u[j] << 16);
-      f[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
-    }
+    r.v = __ldg(p);
   } else {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+#pragma unroll
+    for (int i = 0; i < Raw<V, T>::W; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  return r;
+}
+template <int V, typename T>
+__device__ __forceinline__ Raw<V, T> zero_raw() {
+  Raw<V, T> r;
+  if constexpr (V == 1) {
+    from_f(0.f, &r.v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Raw<V, T>::W; ++i) r.w[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  return r;
+}
+template <int V, typename T>
+__device__ __forceinline__ void to_f32(const Raw<V, T>& r, float* f) {
+  if constexpr (V == 1) {
+    f[0] = to_f(r.v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Raw<V, T>::W; ++i) {
+      const uint32_t u[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 2) {
+          f[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
+          f[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
+        } else {
+          f[4 * i + j] = __uint_as_float(u[j]);
+        }
+      }
+    }
   }
 }
 template <int V, typename T>
-__device__ __forceinline__ void store_v(T* p, const float (&f)[V]) {
+__device__ __forceinline__ void store_v(T* p, const float* f) {
   if constexpr (V == 1) {
     from_f(f[0], p);
   } else if constexpr (sizeof(T) == 2) {
@@ -96,20 +132,64 @@ __device__ __forceinline__ void store_v(T* p, const float (&f)[V]) {
   }
 }
 
-// |v| joins a running maximum that keeps a NaN.
-__device__ __forceinline__ float amax_nan(float m, float v) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
+// Pairs: one instruction for two fp32 operations (sm_100), which is what keeps
+// these kernels bound by memory and not by instruction issue.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
   return r;
 }
-// Non-negative floats and NaN order as their bits do.
-__device__ __forceinline__ float warp_amax(float m) {
-  return __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m)));
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
 }
-__device__ __forceinline__ float warp_sum_f(float v) {
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// max(|a|, |b|, m), keeping a NaN.
+__device__ __forceinline__ float amax2(float a, float b, float m) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(m));
+  return r;
+}
+template <int L>
+__device__ __forceinline__ float amax_all(const float (&y)[L]) {
+  float m = 0.f, m2 = 0.f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  return v;
+  for (int i = 0; i + 3 < L; i += 4) {
+    m = amax2(y[i], y[i + 1], m);
+    m2 = amax2(y[i + 2], y[i + 3], m2);
+  }
+#pragma unroll
+  for (int i = L / 4 * 4; i < L; ++i) m = amax2(y[i], 0.f, m);
+  return amax2(m, m2, 0.f);
+}
+template <int L>
+__device__ __forceinline__ float square_sum(const float (&y)[L]) {
+  uint64_t s = pair(0.f, 0.f), s2 = s;
+#pragma unroll
+  for (int i = 0; i + 3 < L; i += 4) {
+    const uint64_t u = pair(y[i], y[i + 1]), v = pair(y[i + 2], y[i + 3]);
+    s = fma2(u, u, s);
+    s2 = fma2(v, v, s2);
+  }
+  float a, b;
+  unpair(add2(s, s2), a, b);
+  a += b;
+#pragma unroll
+  for (int i = L / 4 * 4; i < L; ++i) a = fmaf(y[i], y[i], a);
+  return a;
 }
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
@@ -125,17 +205,21 @@ __device__ __forceinline__ void row_scale(float amax, float& s, float& inv) {
 }
 // y / s to the nearest integer, ties to even, as the low byte of the sum: |y * inv| < 127.5
 // by the scale's construction.
-__device__ __forceinline__ uint32_t round_byte(float y, float inv) {
-  return __float_as_uint(__fadd_rn(__fmul_rn(y, inv), 12582912.f));
-}
+constexpr float kRound = 12582912.f;  // 1.5 * 2^23
 template <int V>
-__device__ __forceinline__ void store_q(int8_t* p, const float (&y)[V], float inv) {
+__device__ __forceinline__ void store_q(int8_t* p, const float* y, float inv) {
   if constexpr (V == 1) {
-    *p = inv != 0.f ? (int8_t)(round_byte(y[0], inv) & 0xFFu) : (int8_t)0;
+    *p = inv != 0.f ? (int8_t)(__float_as_uint(__fadd_rn(__fmul_rn(y[0], inv), kRound)) & 0xFFu) : (int8_t)0;
   } else {
     uint32_t b[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = round_byte(y[j], inv);
+    for (int j = 0; j < 4; ++j) {
+      float lo, hi;
+      // (as two scalar products: ptxas joins the packed product and sum into one rounding)
+      unpair(add2(pair(__fmul_rn(y[2 * j], inv), __fmul_rn(y[2 * j + 1], inv)), pair(kRound, kRound)), lo, hi);
+      b[2 * j] = __float_as_uint(lo);
+      b[2 * j + 1] = __float_as_uint(hi);
+    }
     uint2 o;
     o.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     o.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
@@ -143,120 +227,264 @@ __device__ __forceinline__ void store_q(int8_t* p, const float (&y)[V], float in
   }
 }
 
-// h of V values at column e of a row (and, with a residual, its store).
-template <int MODE, int V, typename T>
-__device__ __forceinline__ void load_h(const QuantArgs& a, long row, long b, int e, float (&f)[V], bool store) {
-  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx + e;
-  load_v<V, T>(x, f);
-  if constexpr (MODE == kSwiglu) {
-    float u[V];
-    load_v<V, T>(x + a.D, u);
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = silu_mul(f[j], u[j]);
-  } else if constexpr (MODE == kNormRes) {
-    float r[V];
-    load_v<V, T>(reinterpret_cast<const T*>(a.res) + row * a.ldr + e, r);
-    if (a.gate != nullptr) {
-      float g[V];
-      load_v<V, T>(reinterpret_cast<const T*>(a.gate) + b * a.ld_gate + e, g);
-#pragma unroll
-      for (int j = 0; j < V; ++j) f[j] = __fadd_rn(r[j], __fmul_rn(g[j], f[j]));
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) f[j] += r[j];
-    }
-    if (store) store_v<V, T>(reinterpret_cast<T*>(a.h) + row * a.ldh + e, f);
-  }
-}
-// y of V values whose h is in f.
-template <int V, typename T>
-__device__ __forceinline__ void modulate(const QuantArgs& a, long b, int e, float rstd, float (&f)[V]) {
-#pragma unroll
-  for (int j = 0; j < V; ++j) f[j] *= rstd;
-  float t[V];
-  if (a.w != nullptr) {
-    load_v<V, T>(reinterpret_cast<const T*>(a.w) + e, t);
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[j] *= t[j];
-  }
-  if (a.scale != nullptr) {
-    load_v<V, T>(reinterpret_cast<const T*>(a.scale) + b * a.ld_scale + e, t);
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[j] *= 1.f + t[j];
-  }
-  if (a.shift != nullptr) {
-    load_v<V, T>(reinterpret_cast<const T*>(a.shift) + b * a.ld_shift + e, t);
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[j] += t[j];
-  }
-}
-
-// Sum (or NaN-keeping maximum) over the threads of a row: a warp, or the block.
+// Sum, or NaN-keeping maximum, over the lanes of a row (8, 16 or 32 of a warp).
+// Non-negative floats and NaN order as their bits do.
 template <bool MAX>
-__device__ __forceinline__ float row_reduce(float v, int warps, float* smem) {
-  v = MAX ? warp_amax(v) : warp_sum_f(v);
+__device__ __forceinline__ float lane_reduce(float v, int lanes) {
+  if (MAX && lanes == 32) return __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v)));
+  for (int o = lanes / 2; o > 0; o >>= 1) {
+    const float u = __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    if constexpr (MAX) v = __uint_as_float(max(__float_as_uint(v), __float_as_uint(u)));
+    else v += u;
+  }
+  return v;
+}
+// The same over a row that is `warps` warps (the block, if more than one).
+template <bool MAX>
+__device__ __forceinline__ float row_reduce(float v, int lanes, int warps, float* smem) {
+  v = lane_reduce<MAX>(v, lanes);
   if (warps == 1) return v;
   if (threadIdx.x % 32 == 0) smem[threadIdx.x / 32] = v;
   __syncthreads();
   v = threadIdx.x % 32 < warps ? smem[threadIdx.x % 32] : 0.f;
-  return MAX ? warp_amax(v) : warp_sum_f(v);
+  return lane_reduce<MAX>(v, 32);
 }
 
-// One row for each `warps` warps, the row's values in registers: thread t holds
-// N groups of V values, group k at column (k * 32 * warps + t) * V.  warps == 1:
-// each warp of the block has a row of its own and nothing is shared; otherwise
-// the block is one row.  V = 8 needs D % 8 == 0 and 16-byte aligned rows.
+// A row's values in registers: its `per_row` threads (8, 16 or 32 lanes of a warp,
+// or the block) hold N groups of V values each, group k of thread t at column
+// (k * per_row + t) * V.  V = 8 needs D % 8 == 0 and 16-byte aligned rows.  All of a
+// thread's loads are issued before the first is used.
 template <int MODE, typename T, int V, int N>
-__global__ void __launch_bounds__(32 * kMaxWarps) quant_rows_kernel(const QuantArgs a, int warps) {
+__global__ void __launch_bounds__(32 * kMaxWarps) quant_rows_kernel(const QuantArgs a, int lanes, int warps) {
+  constexpr bool NORM = MODE >= kNorm, TWO = MODE == kSwiglu || MODE == kNormRes;
   __shared__ float red[2][32];
-  const int per_row = 32 * warps;
-  const long row = warps == 1 ? (long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : (long)blockIdx.x;
-  if (row >= a.R) return;  // warps == 1: whole warps, no barrier follows
-  const int t = warps == 1 ? threadIdx.x % 32 : threadIdx.x;
-  const long b = MODE >= kNorm ? row / a.rows_per_batch : 0;
-  float y[N][V];
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int e = (k * per_row + t) * V;
-    if (e < a.D) {
-      load_h<MODE, V, T>(a, row, b, e, y[k], true);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) y[k][j] = 0.f;
-    }
-  }
-  if constexpr (MODE >= kNorm) {
-    float ss = 0.f;
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-#pragma unroll
-      for (int j = 0; j < V; ++j) ss += y[k][j] * y[k][j];
-    ss = row_reduce<false>(ss, warps, red[0]);
-    const float rstd = rsqrtf(ss / (float)a.D + a.eps);
+  const int per_row = lanes * warps;
+  const int t = warps == 1 ? threadIdx.x % lanes : threadIdx.x;
+  const long at = warps == 1 ? (long)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes : (long)blockIdx.x;
+  // groups past the end go along with the last row (shuffles need the whole warp) and store nothing
+  const long row = min(at, a.R - 1);
+  const bool live = at < a.R;
+  using R_ = Raw<V, T>;
+  R_ x[N], x2[TWO ? N : 1];
+  {
+    const T* px = reinterpret_cast<const T*>(a.x) + row * a.ldx;
+    const T* p2 = MODE == kSwiglu ? px + a.D : reinterpret_cast<const T*>(a.res) + row * a.ldr;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int e = (k * per_row + t) * V;
-      if (e < a.D) modulate<V, T>(a, b, e, rstd, y[k]);
+      x[k] = e < a.D ? load_raw<V, T>(px + e) : zero_raw<V, T>();
+      if constexpr (TWO) x2[k] = e < a.D ? load_raw<V, T>(p2 + e) : zero_raw<V, T>();
     }
   }
-  float m = 0.f;
+  R_ vw[NORM ? N : 1], vscale[NORM ? N : 1], vshift[NORM ? N : 1], vgate[MODE == kNormRes ? N : 1];
+  if constexpr (NORM) {
+    const long b = row / a.rows_per_batch;
 #pragma unroll
-  for (int k = 0; k < N; ++k)
+    for (int k = 0; k < N; ++k) {
+      const int e = (k * per_row + t) * V;
+      const bool in = e < a.D;
+      vw[k] = in && a.w != nullptr ? load_raw<V, T>(reinterpret_cast<const T*>(a.w) + e) : zero_raw<V, T>();
+      vscale[k] = in && a.scale != nullptr
+                      ? load_raw<V, T>(reinterpret_cast<const T*>(a.scale) + b * a.ld_scale + e)
+                      : zero_raw<V, T>();
+      vshift[k] = in && a.shift != nullptr
+                      ? load_raw<V, T>(reinterpret_cast<const T*>(a.shift) + b * a.ld_shift + e)
+                      : zero_raw<V, T>();
+      if constexpr (MODE == kNormRes)
+        vgate[k] = in && a.gate != nullptr ? load_raw<V, T>(reinterpret_cast<const T*>(a.gate) + b * a.ld_gate + e)
+                                           : zero_raw<V, T>();
+    }
+  }
+  float y[N * V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) m = amax_nan(m, y[k][j]);
-  m = row_reduce<true>(m, warps, red[1]);
+  for (int k = 0; k < N; ++k) {
+    float* const yk = y + k * V;
+    to_f32<V, T>(x[k], yk);
+    if constexpr (TWO) {
+      float f[V];
+      to_f32<V, T>(x2[k], f);
+      if constexpr (MODE == kSwiglu) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) yk[j] = silu_mul(yk[j], f[j]);
+      } else {
+        float g[V];
+        to_f32<V, T>(vgate[k], g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) yk[j] = fmaf(a.gate != nullptr ? g[j] : 1.f, yk[j], f[j]);
+        const int e = (k * per_row + t) * V;
+        if (live && e < a.D) store_v<V, T>(reinterpret_cast<T*>(a.h) + row * a.ldh + e, yk);
+      }
+    }
+  }
+  if constexpr (NORM) {
+    const float ss = row_reduce<false>(square_sum(y), lanes, warps, red[0]);
+    const float rstd = rsqrtf(ss / (float)a.D + a.eps);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      float w[V], sc[V], sh[V];
+      to_f32<V, T>(vw[k], w);
+      to_f32<V, T>(vscale[k], sc);
+      to_f32<V, T>(vshift[k], sh);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float mul = (a.w != nullptr ? w[j] : 1.f) * (1.f + sc[j]);
+        y[k * V + j] = fmaf(y[k * V + j] * rstd, mul, sh[j]);
+      }
+    }
+  }
+  const float m = row_reduce<true>(amax_all(y), lanes, warps, red[1]);
   float s, inv;
   row_scale(m, s, inv);
-  if (t == 0) a.s[row] = s;
+  if (live && t == 0) a.s[row] = s;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const int e = (k * per_row + t) * V;
-    if (e < a.D) store_q<V>(a.q + row * a.ldq + e, y[k], inv);
+    if (live && e < a.D) store_q<V>(a.q + row * a.ldq + e, y + k * V, inv);
+  }
+}
+
+// Many rows of a norm.  A block belongs to one sample (blockIdx.y) and keeps that
+// sample's w * (1 + scale), shift and gate in shared memory as fp32; its row groups
+// (a warp each, or the whole block for a wide row) go over the sample's rows with
+// the next row's loads under the reductions of this one.
+template <int MODE, typename T, int V, int N, bool MULTI>
+__global__ void __launch_bounds__(MULTI ? 32 * kMaxWarps : 128, MULTI ? 1 : 4)
+    norm_sample_kernel(const QuantArgs a, int warps) {
+  constexpr bool TWO = MODE == kNormRes;
+  constexpr int H = V == 8 ? 4 : 1;  // a vector lies in V / H planes, so that 16-byte reads meet no bank twice
+  extern __shared__ __align__(16) float vec[];
+  __shared__ float red[2][32];
+  const int slots = (a.D + V - 1) / V;
+  float* const s_mul = vec;  // each [V / H][slots][H]
+  float* const s_shift = s_mul + slots * V;
+  float* const s_gate = s_shift + slots * V;
+  const long b = blockIdx.y;
+  for (int e = threadIdx.x; e < a.D; e += blockDim.x) {
+    const int at = ((e % V) / H * slots + e / V) * H + e % H;
+    float m = a.w != nullptr ? to_f(reinterpret_cast<const T*>(a.w)[e]) : 1.f;
+    if (a.scale != nullptr) m *= 1.f + to_f(reinterpret_cast<const T*>(a.scale)[b * a.ld_scale + e]);
+    s_mul[at] = m;
+    s_shift[at] = a.shift != nullptr ? to_f(reinterpret_cast<const T*>(a.shift)[b * a.ld_shift + e]) : 0.f;
+    if (TWO) s_gate[at] = a.gate != nullptr ? to_f(reinterpret_cast<const T*>(a.gate)[b * a.ld_gate + e]) : 1.f;
+  }
+  __syncthreads();
+  const int per_row = MULTI ? 32 * warps : 32;
+  const int t = MULTI ? threadIdx.x : threadIdx.x % 32;
+  const int nw = MULTI ? warps : 1;
+  const long stride = (long)gridDim.x * (MULTI ? 1 : 4);
+  auto in = [&](int k) { return (V == 8 && k < N - 1) || (k * per_row + t) * V < a.D; };  // V = 8: N is exact
+  auto vector = [&](const float* v, int k, float* f) {
+    const int slot = min(k * per_row + t, slots - 1);
+#pragma unroll
+    for (int h = 0; h < V / H; ++h) {
+      if constexpr (H == 4) {
+        const float4 q4 = *reinterpret_cast<const float4*>(v + (h * slots + slot) * 4);
+        f[4 * h] = q4.x; f[4 * h + 1] = q4.y; f[4 * h + 2] = q4.z; f[4 * h + 3] = q4.w;
+      } else {
+        f[h] = v[slot];
+      }
+    }
+  };
+  using R_ = Raw<V, T>;
+  R_ x[N], x2[TWO ? N : 1];
+  auto load_row = [&](long row) {
+    const T* px = reinterpret_cast<const T*>(a.x) + row * a.ldx + t * V;
+    const T* p2 = reinterpret_cast<const T*>(a.res) + row * a.ldr + t * V;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      x[k] = in(k) ? load_raw<V, T>(px + k * per_row * V) : zero_raw<V, T>();
+      if constexpr (TWO) x2[k] = in(k) ? load_raw<V, T>(p2 + k * per_row * V) : zero_raw<V, T>();
+    }
+  };
+  long r = (long)blockIdx.x * (MULTI ? 1 : 4) + (MULTI ? 0 : threadIdx.x / 32);
+  if (r < a.rows_per_batch) load_row(b * a.rows_per_batch + r);
+  for (; r < a.rows_per_batch; r += stride) {
+    const long row = b * a.rows_per_batch + r;
+    float y[N * V];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      float* const yk = y + k * V;
+      to_f32<V, T>(x[k], yk);
+      if constexpr (TWO) {
+        float f[V], g[V];
+        to_f32<V, T>(x2[k], f);
+        vector(s_gate, k, g);
+        if constexpr (V == 8) {
+#pragma unroll
+          for (int j = 0; j < V; j += 2)
+            unpair(fma2(pair(g[j], g[j + 1]), pair(yk[j], yk[j + 1]), pair(f[j], f[j + 1])), yk[j], yk[j + 1]);
+        } else {
+          yk[0] = fmaf(g[0], yk[0], f[0]);
+        }
+        if (!in(k)) {  // the clamped slot's gate may be NaN or infinite
+#pragma unroll
+          for (int j = 0; j < V; ++j) yk[j] = 0.f;
+        }
+      }
+    }
+    if (r + stride < a.rows_per_batch) load_row(row + stride);
+    if constexpr (TWO) {
+      T* const h = reinterpret_cast<T*>(a.h) + row * a.ldh + t * V;
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (in(k)) store_v<V, T>(h + k * per_row * V, y + k * V);
+    }
+    const float ss = row_reduce<false>(square_sum(y), 32, nw, red[0]);
+    const float rstd = rsqrtf(ss / (float)a.D + a.eps);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      float* const yk = y + k * V;
+      float mul[V], sh[V];
+      vector(s_mul, k, mul);
+      vector(s_shift, k, sh);
+      if constexpr (V == 8) {
+#pragma unroll
+        for (int j = 0; j < V; j += 2)
+          unpair(fma2(mul2(pair(yk[j], yk[j + 1]), pair(rstd, rstd)), pair(mul[j], mul[j + 1]), pair(sh[j], sh[j + 1])),
+                 yk[j], yk[j + 1]);
+      } else {
+        yk[0] = fmaf(yk[0] * rstd, mul[0], sh[0]);
+      }
+      if (!in(k)) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) yk[j] = 0.f;
+      }
+    }
+    const float m = row_reduce<true>(amax_all(y), 32, nw, red[1]);
+    float s, inv;
+    row_scale(m, s, inv);
+    if (t == 0) a.s[row] = s;
+    int8_t* const q = a.q + row * a.ldq + t * V;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (in(k)) store_q<V>(q + k * per_row * V, y + k * V, inv);
   }
 }
 
 // Rows too wide for the registers of one block: the block goes over the row
 // once for each reduction and once for the rounding.
+template <int MODE, typename T>
+__device__ __forceinline__ float wide_h(const QuantArgs& a, long row, long b, int e, bool store) {
+  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx + e;
+  float f = to_f(*x);
+  if constexpr (MODE == kSwiglu) f = silu_mul(f, to_f(x[a.D]));
+  if constexpr (MODE == kNormRes) {
+    const float g = a.gate != nullptr ? to_f(reinterpret_cast<const T*>(a.gate)[b * a.ld_gate + e]) : 1.f;
+    f = fmaf(g, f, to_f(reinterpret_cast<const T*>(a.res)[row * a.ldr + e]));
+    if (store) from_f(f, reinterpret_cast<T*>(a.h) + row * a.ldh + e);
+  }
+  return f;
+}
+template <int MODE, typename T>
+__device__ __forceinline__ float wide_y(const QuantArgs& a, long row, long b, int e, float rstd) {
+  float f = wide_h<MODE, T>(a, row, b, e, false);
+  if constexpr (MODE >= kNorm) {
+    float mul = a.w != nullptr ? to_f(reinterpret_cast<const T*>(a.w)[e]) : 1.f;
+    if (a.scale != nullptr) mul *= 1.f + to_f(reinterpret_cast<const T*>(a.scale)[b * a.ld_scale + e]);
+    f = fmaf(f * rstd, mul, a.shift != nullptr ? to_f(reinterpret_cast<const T*>(a.shift)[b * a.ld_shift + e]) : 0.f);
+  }
+  return f;
+}
 template <int MODE, typename T>
 __global__ void __launch_bounds__(512) quant_wide_kernel(const QuantArgs a) {
   __shared__ float red[2][32];
@@ -267,81 +495,184 @@ __global__ void __launch_bounds__(512) quant_wide_kernel(const QuantArgs a) {
   if constexpr (MODE >= kNorm) {
     float ss = 0.f;
     for (int e = threadIdx.x; e < a.D; e += blockDim.x) {
-      float f[1];
-      load_h<MODE, 1, T>(a, row, b, e, f, true);
-      ss += f[0] * f[0];
+      const float f = wide_h<MODE, T>(a, row, b, e, true);
+      ss += f * f;
     }
-    ss = row_reduce<false>(ss, warps, red[0]);
+    ss = row_reduce<false>(ss, 32, warps, red[0]);
     rstd = rsqrtf(ss / (float)a.D + a.eps);
   }
   float m = 0.f;
-  for (int e = threadIdx.x; e < a.D; e += blockDim.x) {
-    float f[1];
-    load_h<MODE, 1, T>(a, row, b, e, f, false);
-    if constexpr (MODE >= kNorm) modulate<1, T>(a, b, e, rstd, f);
-    m = amax_nan(m, f[0]);
-  }
-  m = row_reduce<true>(m, warps, red[1]);
+  for (int e = threadIdx.x; e < a.D; e += blockDim.x) m = amax2(wide_y<MODE, T>(a, row, b, e, rstd), 0.f, m);
+  m = row_reduce<true>(m, 32, warps, red[1]);
   float s, inv;
   row_scale(m, s, inv);
   if (threadIdx.x == 0) a.s[row] = s;
   for (int e = threadIdx.x; e < a.D; e += blockDim.x) {
-    float f[1];
-    load_h<MODE, 1, T>(a, row, b, e, f, false);
-    if constexpr (MODE >= kNorm) modulate<1, T>(a, b, e, rstd, f);
-    store_q<1>(a.q + row * a.ldq + e, f, inv);
+    const float y[1] = {wide_y<MODE, T>(a, row, b, e, rstd)};
+    store_q<1>(a.q + row * a.ldq + e, y, inv);
+  }
+}
+
+// q * s.  Rows of whole 16-byte groups: a thread turns 16 values of one row into
+// 32 (or 64) bytes; else neighbouring lanes take neighbouring values.
+template <typename T>
+__global__ void __launch_bounds__(256) dequant_vec_kernel(const int8_t* __restrict__ q, long ldq,
+                                                          const float* __restrict__ s, long groups, int per_row,
+                                                          T* __restrict__ out) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= groups) return;
+  const long row = i / per_row;
+  const int e = (int)(i - row * per_row) * 16;
+  const uint4 v = *reinterpret_cast<const uint4*>(q + row * ldq + e);
+  const float sc = s[row];
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (float)(int8_t)(w[2 * g + j / 4] >> (8 * (j % 4))) * sc;
+    store_v<8, T>(out + i * 16 + g * 8, f);
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* __restrict__ q, long ldq,
+                                                           const float* __restrict__ s, int D, T* __restrict__ out) {
+  const long row = blockIdx.x;
+  const float sc = s[row];
+  for (int e0 = threadIdx.x; e0 < D; e0 += 4 * 256) {
+    int8_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = e0 + j * 256 < D ? q[row * ldq + e0 + j * 256] : (int8_t)0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (e0 + j * 256 < D) from_f((float)v[j] * sc, out + row * D + e0 + j * 256);
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* __restrict__ q, long ldq,
-                                                           const float* __restrict__ s, long R, int D,
-                                                           T* __restrict__ out, long ldo) {
-  for (long row = blockIdx.x; row < R; row += gridDim.x) {
-    const float sc = s[row];
-    for (int e = threadIdx.x; e < D; e += blockDim.x) from_f((float)q[row * ldq + e] * sc, out + row * ldo + e);
-  }
+void launch_dequant(const int8_t* q, long ldq, const float* s, long R, int D, T* out, cudaStream_t stream) {
+  const bool vec = D % 16 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (R == 1 || ldq % 16 == 0);
+  const long blocks = vec ? (R * (D / 16) + 255) / 256 : R;
+  TORCH_CHECK(blocks <= 0x7FFFFFFFL, "dequant_rows: too many rows");
+  if (vec) dequant_vec_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>(q, ldq, s, R * (D / 16), D / 16, out);
+  else dequant_rows_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>(q, ldq, s, D, out);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  count_launch();
 }
 
 template <int MODE, typename T, int V, int N>
-void launch_n(const QuantArgs& a, int warps, cudaStream_t stream) {
-  const int rows_per_block = warps == 1 ? 4 : 1;
-  const long grid = (a.R + rows_per_block - 1) / rows_per_block;
-  TORCH_CHECK(grid <= 0x7FFFFFFFL, "harp quant: too many rows");
-  quant_rows_kernel<MODE, T, V, N><<<(unsigned)grid, 32 * warps * rows_per_block, 0, stream>>>(a, warps);
+void launch_few(const QuantArgs& a, int lanes, int warps, cudaStream_t stream) {
+  const int threads = warps == 1 ? 128 : 32 * warps;
+  const int per_block = warps == 1 ? threads / lanes : 1;
+  const long blocks = (a.R + per_block - 1) / per_block;
+  TORCH_CHECK(blocks <= 0x7FFFFFFFL, "harp quant: too many rows");
+  quant_rows_kernel<MODE, T, V, N><<<(unsigned)blocks, threads, 0, stream>>>(a, lanes, warps);
+}
+
+template <int MODE, typename T, int V, int N, bool MULTI>
+void launch_sample(const QuantArgs& a, int warps, size_t smem, cudaStream_t stream) {
+  auto kern = norm_sample_kernel<MODE, T, V, N, MULTI>;
+  const int threads = MULTI ? 32 * warps : 128, per_block = MULTI ? 1 : 4;
+  static std::once_flag once;
+  std::call_once(once, [&] {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kVecSmem));
+  });
+  int n = 0;
+  C10_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem));
+  const long samples = a.R / a.rows_per_batch;
+  const long most = (a.rows_per_batch + per_block - 1) / per_block;
+  const long blocks = std::max<long>(1, std::min<long>(most, (long)std::max(1, n) * num_sms() / samples));
+  kern<<<dim3((unsigned)blocks, (unsigned)samples), threads, smem, stream>>>(a, warps);
+}
+
+// The least warps that hold a row in N groups a thread with few idle slots.
+struct RowShape {
+  int warps, n;
+};
+RowShape fewest_warps(int groups, int most) {
+  RowShape best = {0, 0};
+  double used = 0.0;
+  for (int w = 1; w <= kMaxWarps; ++w) {
+    const int n = (groups + 32 * w - 1) / (32 * w);
+    const double u = (double)groups / (32.0 * w * n);
+    if (n <= most && u > used * 1.02) { used = u; best = {w, n}; }
+  }
+  return best;
 }
 
 template <int MODE, typename T>
 void launch(const QuantArgs& a, bool vec, cudaStream_t stream) {
-  // Groups of V values for each thread: the fewest warps that hold the row with
-  // the fewest idle slots.
-  const int V = vec ? 8 : 1, most = vec ? 5 : 16;
+  const int V = vec ? 8 : 1;
   const int groups = (a.D + V - 1) / V;
-  int warps = 0, n = 0;
-  double best = 0.0;
-  for (int w = 1; w <= kMaxWarps; ++w) {
-    const int need = (groups + 32 * w - 1) / (32 * w);
-    if (need > most) continue;
-    const double used = (double)groups / (32.0 * w * need);
-    if (used > best * 1.02) { best = used; warps = w; n = need; }
-  }
-  if (warps == 0) {
-    TORCH_CHECK(a.R <= 0x7FFFFFFFL, "harp quant: too many rows");
-    quant_wide_kernel<MODE, T><<<(unsigned)a.R, 512, 0, stream>>>(a);
-  } else if (vec) {
-    switch (n) {
-      case 1: launch_n<MODE, T, 8, 1>(a, warps, stream); break;
-      case 2: launch_n<MODE, T, 8, 2>(a, warps, stream); break;
-      case 3: launch_n<MODE, T, 8, 3>(a, warps, stream); break;
-      case 4: launch_n<MODE, T, 8, 4>(a, warps, stream); break;
-      default: launch_n<MODE, T, 8, 5>(a, warps, stream); break;
+  const RowShape many = fewest_warps(groups, vec ? 5 : 16);
+  const long samples = MODE >= kNorm ? a.R / a.rows_per_batch : 1;
+  bool done = false;
+  // Many rows: few warps a row, several groups a thread.
+  if (many.warps > 0 && a.R * many.warps > 8L * num_sms()) {
+    done = true;
+    if constexpr (MODE >= kNorm) {
+      const size_t smem = (size_t)groups * V * 4 * (MODE == kNormRes ? 3 : 2);
+      if (smem <= kVecSmem && samples <= 65535 && a.rows_per_batch >= 8) {
+#define HARP_SAMPLE(V_, N_)                                                                   \
+  (many.warps == 1 ? launch_sample<MODE, T, V_, N_, false>(a, many.warps, smem, stream)       \
+                   : launch_sample<MODE, T, V_, N_, true>(a, many.warps, smem, stream))
+        if (vec) {
+          switch (many.n) {
+            case 1: HARP_SAMPLE(8, 1); break;
+            case 2: HARP_SAMPLE(8, 2); break;
+            case 3: HARP_SAMPLE(8, 3); break;
+            case 4: HARP_SAMPLE(8, 4); break;
+            default: HARP_SAMPLE(8, 5); break;
+          }
+        } else if (many.n <= 4) {
+          HARP_SAMPLE(1, 4);
+        } else if (many.n <= 8) {
+          HARP_SAMPLE(1, 8);
+        } else {
+          HARP_SAMPLE(1, 16);
+        }
+#undef HARP_SAMPLE
+      } else {
+        done = false;
+      }
+    } else if (vec) {
+      const int lanes = groups <= 8 ? 8 : groups <= 16 ? 16 : 32;
+      switch (many.n) {
+        case 1: launch_few<MODE, T, 8, 1>(a, lanes, many.warps, stream); break;
+        case 2: launch_few<MODE, T, 8, 2>(a, 32, many.warps, stream); break;
+        case 3: launch_few<MODE, T, 8, 3>(a, 32, many.warps, stream); break;
+        case 4: launch_few<MODE, T, 8, 4>(a, 32, many.warps, stream); break;
+        default: launch_few<MODE, T, 8, 5>(a, 32, many.warps, stream); break;
+      }
+    } else if (many.n <= 4) {
+      launch_few<MODE, T, 1, 4>(a, 32, many.warps, stream);
+    } else if (many.n <= 8) {
+      launch_few<MODE, T, 1, 8>(a, 32, many.warps, stream);
+    } else {
+      launch_few<MODE, T, 1, 16>(a, 32, many.warps, stream);
     }
-  } else if (n <= 4) {
-    launch_n<MODE, T, 1, 4>(a, warps, stream);
-  } else if (n <= 8) {
-    launch_n<MODE, T, 1, 8>(a, warps, stream);
-  } else {
-    launch_n<MODE, T, 1, 16>(a, warps, stream);
+  }
+  if (!done) {
+    // Few rows: latency counts, so as many warps as the row has groups for.
+    const int n = (groups + 32 * kMaxWarps - 1) / (32 * kMaxWarps);
+    const int lanes = vec && groups <= 8 ? 8 : vec && groups <= 16 ? 16 : 32;
+    auto warps = [&](int per_thread) { return std::max(1, (groups + 32 * per_thread - 1) / (32 * per_thread)); };
+    if (vec && n == 1) {
+      launch_few<MODE, T, 8, 1>(a, lanes, warps(1), stream);
+    } else if (vec && n == 2) {
+      launch_few<MODE, T, 8, 2>(a, 32, warps(2), stream);
+    } else if (vec && n <= 5) {
+      launch_few<MODE, T, 8, 5>(a, 32, warps(5), stream);
+    } else if (!vec && n <= 4) {
+      launch_few<MODE, T, 1, 4>(a, 32, warps(4), stream);
+    } else if (!vec && n <= 8) {
+      launch_few<MODE, T, 1, 8>(a, 32, warps(8), stream);
+    } else if (!vec && n <= 16) {
+      launch_few<MODE, T, 1, 16>(a, 32, warps(16), stream);
+    } else {
+      TORCH_CHECK(a.R <= 0x7FFFFFFFL, "harp quant: too many rows");
+      quant_wide_kernel<MODE, T><<<(unsigned)a.R, 512, 0, stream>>>(a);
+    }
   }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   count_launch();
@@ -488,15 +819,9 @@ at::Tensor dequant_rows(const at::Tensor& q, const at::Tensor& s, bool f32) {
   at::Tensor out(at::detail::empty_cuda({R, D}, f32 ? at::kFloat : at::kBFloat16, q.device(), c10::nullopt));
   if (R == 0 || D == 0) return out;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  const unsigned grid = (unsigned)std::min<long>(R, 1L << 20);
   const int8_t* qp = reinterpret_cast<const int8_t*>(q.data_ptr());
-  if (f32)
-    dequant_rows_kernel<float><<<grid, 256, 0, stream>>>(qp, q.stride(0), s.data_ptr<float>(), R, (int)D, out.data_ptr<float>(), D);
-  else
-    dequant_rows_kernel<bf16><<<grid, 256, 0, stream>>>(qp, q.stride(0), s.data_ptr<float>(), R, (int)D,
-                                                        reinterpret_cast<bf16*>(out.data_ptr()), D);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  count_launch();
+  if (f32) launch_dequant<float>(qp, q.stride(0), s.data_ptr<float>(), R, (int)D, out.data_ptr<float>(), stream);
+  else launch_dequant<bf16>(qp, q.stride(0), s.data_ptr<float>(), R, (int)D, reinterpret_cast<bf16*>(out.data_ptr()), stream);
   return out;
 }
 
