@@ -30,7 +30,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import asdict, dataclass
-from typing import List, Optional, Sequence, Tuple
+from typing import TYPE_CHECKING, List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn as nn
@@ -38,6 +38,9 @@ import torch.nn as nn
 from ..ops import functional as Fn
 from ..ops.modules import LinearFunction, SiLUFunction
 from ..parallel.sequence import SPContext, qkv_attention_backward, qkv_attention_forward
+
+if TYPE_CHECKING:
+    from .dit_int8 import DiTInt8
 
 
 # ---------------------------------------------------------------------------
@@ -463,10 +466,20 @@ class DiT(nn.Module):
         c = self.t_embedder(t * 1000.0)
         c_silu = SiLUFunction.apply(c)
         freqs = self.freqs_for(h_tok, w_tok, L, lo, hi, h.device)
+        out = self.final_layer(self.run_blocks(h, c_silu, freqs, sp), c_silu)
+        return out[:, : img_hi - img_lo], img_lo, img_hi
+
+    def run_blocks(self, h: torch.Tensor, c_silu: torch.Tensor, freqs: torch.Tensor, sp: SPContext) -> torch.Tensor:
         for blk in self.blocks:
             h = blk(h, c_silu, freqs, sp)
-        out = self.final_layer(h, c_silu)
-        return out[:, : img_hi - img_lo], img_lo, img_hi
+        return h
+
+    def int8(self) -> "DiTInt8":
+        """This model for inference with its blocks' products in 8-bit integers
+        (harp_b200.models.dit_int8); embedders and final layer are shared."""
+        from .dit_int8 import DiTInt8
+
+        return DiTInt8(self)
 
     def forward(self, latent: torch.Tensor, text: torch.Tensor, t: torch.Tensor, sp: Optional[SPContext] = None):
         """Full-sequence convenience forward (single SP rank): returns the

@@ -97,6 +97,46 @@ def replace_linear_with_kplinear(model: nn.Module, kplinear_class=kpLinear) -> n
     return model
 
 
+class Int8Linear(nn.Module):
+    """Inference linear layer in 8-bit integers: the weight [out, in] in int8 with a scale
+    for each output channel, the input quantised per row (``functional.quant_rows``), the
+    product on ``functional.gemm_s8``; bf16 or fp32 input, output in the input's type.
+    No gradients."""
+
+    def __init__(self, in_features, out_features, bias=True, device=None):
+        super().__init__()
+        self.in_features, self.out_features = in_features, out_features
+        self.register_buffer("weight_q", torch.zeros(out_features, in_features, device=device, dtype=torch.int8))
+        self.register_buffer("weight_scale", torch.ones(out_features, device=device))
+        self.register_buffer("bias", torch.zeros(out_features, device=device) if bias else None)
+
+    @classmethod
+    @torch.no_grad()
+    def from_weight(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "Int8Linear":
+        m = cls(weight.shape[1], weight.shape[0], bias=False, device="meta")
+        m.weight_q, m.weight_scale = Fn.quant_rows(weight.detach())
+        m.bias = bias.detach().clone() if bias is not None else None
+        return m
+
+    @classmethod
+    def from_linear(cls, linear: nn.Module) -> "Int8Linear":
+        """From an nn.Linear / kpLinear."""
+        return cls.from_weight(linear.weight, linear.bias)
+
+    def dequantized(self, dtype=torch.bfloat16) -> torch.Tensor:
+        """The weight that the layer multiplies with, [out, in]."""
+        return Fn.dequant_rows(self.weight_q, self.weight_scale, dtype)
+
+    def rows(self, q: torch.Tensor, s: torch.Tensor, out_dtype=torch.bfloat16) -> torch.Tensor:
+        """The product for rows that are already in 8 bits."""
+        return Fn.gemm_s8(q, s, self.weight_q, self.weight_scale, bias=self.bias, out_dtype=out_dtype)
+
+    @torch.no_grad()
+    def forward(self, x):
+        q, s = Fn.quant_rows(x.reshape(-1, x.shape[-1]))
+        return self.rows(q, s, x.dtype).view(*x.shape[:-1], self.out_features)
+
+
 # ---------------------------------------------------------------------------
 # RMSNorm (optional affine weight)
 # ---------------------------------------------------------------------------

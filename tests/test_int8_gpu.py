@@ -324,3 +324,68 @@ def test_refusals():
             f()
             raise AssertionError(f"case {i} was taken")
     torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------------------
+# the layer and the model that use them
+# ---------------------------------------------------------------------------
+def test_int8_linear_cuda_matches_cpu():
+    """Same bits in, exact products: outputs differ by the fp32 rounding of the last step only."""
+    from harp_b200.ops.modules import Int8Linear, kpLinear
+
+    torch.manual_seed(0)
+    lin = kpLinear(200, 136, dtype=torch.float32)
+    x = torch.randn(3, 50, 200)
+    ref = Int8Linear.from_linear(lin)(x)
+    out = Int8Linear.from_linear(lin.cuda())(x.cuda())
+    assert out.shape == ref.shape and ((out.cpu() - ref).abs() <= 2.0 ** -21 * (ref.abs() + 1)).all()
+    xs = x.cuda().transpose(0, 1)  # not contiguous
+    assert torch.equal(Int8Linear.from_linear(lin)(xs), out.transpose(0, 1))
+
+
+def _dit(seed=0):
+    from harp_b200.models import dit as D
+
+    torch.manual_seed(seed)
+    m = D.DiT(D.PRESETS["small"])
+    with torch.no_grad():
+        for n, p in m.named_parameters():
+            p.normal_(0, 0.02 if "adaLN" in n else 0.05)
+            if "norm" in n:
+                p.add_(1.0)
+    return m.bfloat16()
+
+
+@pytest.mark.parametrize("B,L,T", [(2, 16, 32), (1, 8, 5), (3, 34, 77)])
+def test_dit_int8_cuda_matches_cpu(B, L, T):
+    """The same model run through the CPU restatements; bf16 activations, as in the other models' test."""
+    import copy
+
+    m = _dit()
+    g = torch.Generator().manual_seed(1)
+    lat = torch.randn(B, 16, L, L, generator=g).bfloat16()
+    text = torch.randn(B, T, 384, generator=g).bfloat16()
+    t = torch.rand(B, generator=g)
+    ref = m.int8()(lat, text, t).float()
+    q = copy.deepcopy(m).cuda().int8()
+    out = q(lat.cuda(), text.cuda(), t.cuda())
+    torch.cuda.synchronize()
+    errors.check(out.device)
+    assert ((out.float().cpu() - ref).norm() / ref.norm()).item() < 3e-2
+    # and it follows the bf16 model (about 1 % a product)
+    with torch.no_grad():
+        full = m.cuda()(lat.cuda(), text.cuda(), t.cuda())
+    assert ((out - full).float().norm() / full.float().norm()).item() < 6e-2
+
+
+def test_sampling_with_the_int8_dit():
+    from harp_b200.inference import batch_image_inference
+
+    m = _dit().cuda()
+    g = torch.Generator().manual_seed(2)
+    emb = [torch.randn(32, 384, generator=g).bfloat16().cuda() for _ in range(2)]
+    lat = torch.randn(2, 16, 16, 16, generator=g).cuda()
+    kw = dict(prompt_embeds=emb, height=128, width=128, num_inference_steps=4, initial_latents=lat)
+    ref = batch_image_inference(m, **kw)["images"].float()
+    out = batch_image_inference(m.int8(), **kw)["images"].float()
+    assert torch.isfinite(out).all() and ((out - ref).norm() / ref.norm()).item() < 6e-2
