@@ -799,7 +799,15 @@ Plan pick(const S8Args& a) {
 
 template <typename OUT>
 void dispatch(const S8Args& a, bool c_tma, cudaStream_t stream) {
-  const Plan p = pick(a);
+  // the estimate takes about a microsecond on the host, so the plans of the sizes at hand are kept
+  struct Known {
+    int M = -1, N = -1, K = -1;
+    Plan p = {};
+  };
+  static thread_local Known known[64];
+  Known& k = known[((unsigned)a.M * 7u + (unsigned)a.N * 31u + (unsigned)a.K * 131u) % 64u];
+  if (k.M != a.M || k.N != a.N || k.K != a.K) k = {a.M, a.N, a.K, pick(a)};
+  const Plan p = k.p;
   switch (p.pair_bn) {
     case 256: launch_pair<256, OUT>(a, c_tma, stream); return;
     case 192: launch_pair<192, OUT>(a, c_tma, stream); return;

@@ -67,54 +67,60 @@ __device__ __forceinline__ float to_f(bf16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void from_f(float v, float* p) { *p = v; }
 __device__ __forceinline__ void from_f(float v, bf16* p) { *p = __float2bfloat16(v); }
 
-// V consecutive values as they are stored (V = 8: 16-byte aligned), and as fp32.
+// V consecutive values (1, 2 or 8) as they are stored, aligned to their size or to
+// 16 bytes, and as fp32.
+template <int BYTES>
+struct Words {
+  uint4 v[BYTES / 16];
+};
+template <>
+struct Words<2> { uint16_t v[1]; };
+template <>
+struct Words<4> { uint32_t v[1]; };
+template <>
+struct Words<8> { uint2 v[1]; };
 template <int V, typename T>
-struct Raw {
-  static constexpr int W = V * (int)sizeof(T) >= 16 ? V * (int)sizeof(T) / 16 : 1;
-  uint4 w[W];
-};
-template <typename T>
-struct Raw<1, T> {
-  T v;
-};
+using Raw = Words<V * (int)sizeof(T)>;
+
 template <int V, typename T>
 __device__ __forceinline__ Raw<V, T> load_raw(const T* p) {
   Raw<V, T> r;
-  if constexpr (V == 1) {
-    r.v = __ldg(p);
-  } else {
+  using E = std::remove_reference_t<decltype(r.v[0])>;
 #pragma unroll
-    for (int i = 0; i < Raw<V, T>::W; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-  }
+  for (int i = 0; i < (int)(sizeof(r.v) / sizeof(E)); ++i) r.v[i] = __ldg(reinterpret_cast<const E*>(p) + i);
+  return r;
+}
+// Values of a row, which nothing reads again: first to leave the caches, so that
+// they do not push out what is being written (norm of 17408 x 1152 with a residual:
+// 25.9 us, 30.6 without).
+template <int V, typename T>
+__device__ __forceinline__ Raw<V, T> load_once(const T* p) {
+  Raw<V, T> r;
+  using E = std::remove_reference_t<decltype(r.v[0])>;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(r.v) / sizeof(E)); ++i) r.v[i] = __ldcs(reinterpret_cast<const E*>(p) + i);
   return r;
 }
 template <int V, typename T>
 __device__ __forceinline__ Raw<V, T> zero_raw() {
   Raw<V, T> r;
-  if constexpr (V == 1) {
-    from_f(0.f, &r.v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < Raw<V, T>::W; ++i) r.w[i] = make_uint4(0u, 0u, 0u, 0u);
-  }
+  memset(&r, 0, sizeof(r));
   return r;
 }
 template <int V, typename T>
 __device__ __forceinline__ void to_f32(const Raw<V, T>& r, float* f) {
-  if constexpr (V == 1) {
-    f[0] = to_f(r.v);
+  if constexpr (sizeof(T) == 2 && V == 1) {
+    f[0] = __uint_as_float((uint32_t)r.v[0] << 16);
   } else {
+    uint32_t u[sizeof(r) / 4];
+    memcpy(u, &r, sizeof(r));
 #pragma unroll
-    for (int i = 0; i < Raw<V, T>::W; ++i) {
-      const uint32_t u[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(T) == 2) {
-          f[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
-          f[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
-        } else {
-          f[4 * i + j] = __uint_as_float(u[j]);
-        }
+    for (int i = 0; i < (int)(sizeof(r) / 4); ++i) {
+      if constexpr (sizeof(T) == 2) {
+        f[2 * i] = __uint_as_float(u[i] << 16);
+        f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+      } else {
+        f[i] = __uint_as_float(u[i]);
       }
     }
   }
@@ -123,6 +129,9 @@ template <int V, typename T>
 __device__ __forceinline__ void store_v(T* p, const float* f) {
   if constexpr (V == 1) {
     from_f(f[0], p);
+  } else if constexpr (V == 2) {
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(f[0], f[1]);
+    else *reinterpret_cast<float2*>(p) = make_float2(f[0], f[1]);
   } else if constexpr (sizeof(T) == 2) {
     *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
                                               pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
@@ -210,6 +219,10 @@ template <int V>
 __device__ __forceinline__ void store_q(int8_t* p, const float* y, float inv) {
   if constexpr (V == 1) {
     *p = inv != 0.f ? (int8_t)(__float_as_uint(__fadd_rn(__fmul_rn(y[0], inv), kRound)) & 0xFFu) : (int8_t)0;
+  } else if constexpr (V == 2) {
+    const uint32_t b0 = __float_as_uint(__fadd_rn(__fmul_rn(y[0], inv), kRound));
+    const uint32_t b1 = __float_as_uint(__fadd_rn(__fmul_rn(y[1], inv), kRound));
+    *reinterpret_cast<uint16_t*>(p) = inv != 0.f ? (uint16_t)__byte_perm(b0, b1, 0x0040) : (uint16_t)0;
   } else {
     uint32_t b[8];
 #pragma unroll
@@ -252,7 +265,8 @@ __device__ __forceinline__ float row_reduce(float v, int lanes, int warps, float
 
 // A row's values in registers: its `per_row` threads (8, 16 or 32 lanes of a warp,
 // or the block) hold N groups of V values each, group k of thread t at column
-// (k * per_row + t) * V.  V = 8 needs D % 8 == 0 and 16-byte aligned rows.  All of a
+// (k * per_row + t) * V.  V = 8 needs D % 8 == 0 and 16-byte aligned rows, V = 2 an even
+// D and rows aligned to two values.  All of a
 // thread's loads are issued before the first is used.
 template <int MODE, typename T, int V, int N>
 __global__ void __launch_bounds__(32 * kMaxWarps) quant_rows_kernel(const QuantArgs a, int lanes, int warps) {
@@ -272,8 +286,8 @@ __global__ void __launch_bounds__(32 * kMaxWarps) quant_rows_kernel(const QuantA
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int e = (k * per_row + t) * V;
-      x[k] = e < a.D ? load_raw<V, T>(px + e) : zero_raw<V, T>();
-      if constexpr (TWO) x2[k] = e < a.D ? load_raw<V, T>(p2 + e) : zero_raw<V, T>();
+      x[k] = e < a.D ? load_once<V, T>(px + e) : zero_raw<V, T>();
+      if constexpr (TWO) x2[k] = e < a.D ? load_once<V, T>(p2 + e) : zero_raw<V, T>();
     }
   }
   R_ vw[NORM ? N : 1], vscale[NORM ? N : 1], vshift[NORM ? N : 1], vgate[MODE == kNormRes ? N : 1];
@@ -348,10 +362,10 @@ __global__ void __launch_bounds__(32 * kMaxWarps) quant_rows_kernel(const QuantA
 // (a warp each, or the whole block for a wide row) go over the sample's rows with
 // the next row's loads under the reductions of this one.
 template <int MODE, typename T, int V, int N, bool MULTI>
-__global__ void __launch_bounds__(MULTI ? 32 * kMaxWarps : 128, MULTI ? 1 : 4)
+__global__ void __launch_bounds__(MULTI ? 32 * kMaxWarps : 128, MULTI ? 1 : MODE == kNormRes ? 3 : 4)
     norm_sample_kernel(const QuantArgs a, int warps) {
   constexpr bool TWO = MODE == kNormRes;
-  constexpr int H = V == 8 ? 4 : 1;  // a vector lies in V / H planes, so that 16-byte reads meet no bank twice
+  constexpr int H = V == 8 ? 4 : V;  // a vector lies in V / H planes, so that wide reads meet no bank twice
   extern __shared__ __align__(16) float vec[];
   __shared__ float red[2][32];
   const int slots = (a.D + V - 1) / V;
@@ -359,15 +373,6 @@ __global__ void __launch_bounds__(MULTI ? 32 * kMaxWarps : 128, MULTI ? 1 : 4)
   float* const s_shift = s_mul + slots * V;
   float* const s_gate = s_shift + slots * V;
   const long b = blockIdx.y;
-  for (int e = threadIdx.x; e < a.D; e += blockDim.x) {
-    const int at = ((e % V) / H * slots + e / V) * H + e % H;
-    float m = a.w != nullptr ? to_f(reinterpret_cast<const T*>(a.w)[e]) : 1.f;
-    if (a.scale != nullptr) m *= 1.f + to_f(reinterpret_cast<const T*>(a.scale)[b * a.ld_scale + e]);
-    s_mul[at] = m;
-    s_shift[at] = a.shift != nullptr ? to_f(reinterpret_cast<const T*>(a.shift)[b * a.ld_shift + e]) : 0.f;
-    if (TWO) s_gate[at] = a.gate != nullptr ? to_f(reinterpret_cast<const T*>(a.gate)[b * a.ld_gate + e]) : 1.f;
-  }
-  __syncthreads();
   const int per_row = MULTI ? 32 * warps : 32;
   const int t = MULTI ? threadIdx.x : threadIdx.x % 32;
   const int nw = MULTI ? warps : 1;
@@ -380,8 +385,11 @@ __global__ void __launch_bounds__(MULTI ? 32 * kMaxWarps : 128, MULTI ? 1 : 4)
       if constexpr (H == 4) {
         const float4 q4 = *reinterpret_cast<const float4*>(v + (h * slots + slot) * 4);
         f[4 * h] = q4.x; f[4 * h + 1] = q4.y; f[4 * h + 2] = q4.z; f[4 * h + 3] = q4.w;
+      } else if constexpr (H == 2) {
+        const float2 q2 = *reinterpret_cast<const float2*>(v + slot * 2);
+        f[0] = q2.x; f[1] = q2.y;
       } else {
-        f[h] = v[slot];
+        f[0] = v[slot];
       }
     }
   };
@@ -392,12 +400,47 @@ __global__ void __launch_bounds__(MULTI ? 32 * kMaxWarps : 128, MULTI ? 1 : 4)
     const T* p2 = reinterpret_cast<const T*>(a.res) + row * a.ldr + t * V;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      x[k] = in(k) ? load_raw<V, T>(px + k * per_row * V) : zero_raw<V, T>();
-      if constexpr (TWO) x2[k] = in(k) ? load_raw<V, T>(p2 + k * per_row * V) : zero_raw<V, T>();
+      x[k] = in(k) ? load_once<V, T>(px + k * per_row * V) : zero_raw<V, T>();
+      if constexpr (TWO) x2[k] = in(k) ? load_once<V, T>(p2 + k * per_row * V) : zero_raw<V, T>();
     }
   };
   long r = (long)blockIdx.x * (MULTI ? 1 : 4) + (MULTI ? 0 : threadIdx.x / 32);
   if (r < a.rows_per_batch) load_row(b * a.rows_per_batch + r);
+  // the sample's vectors, while the first rows are on their way
+#pragma unroll 2
+  for (int slot = threadIdx.x; slot < slots; slot += blockDim.x) {
+    const int e = slot * V;
+    R_ w, sc, sh, g;
+    if (a.w != nullptr) w = load_raw<V, T>(reinterpret_cast<const T*>(a.w) + e);
+    if (a.scale != nullptr) sc = load_raw<V, T>(reinterpret_cast<const T*>(a.scale) + b * a.ld_scale + e);
+    if (a.shift != nullptr) sh = load_raw<V, T>(reinterpret_cast<const T*>(a.shift) + b * a.ld_shift + e);
+    if (TWO && a.gate != nullptr) g = load_raw<V, T>(reinterpret_cast<const T*>(a.gate) + b * a.ld_gate + e);
+    float f[V], m[V];
+    auto put = [&](float* v, const float* f) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[(j / H * slots + slot) * H + j % H] = f[j];
+    };
+#pragma unroll
+    for (int j = 0; j < V; ++j) m[j] = 1.f;
+    if (a.w != nullptr) to_f32<V, T>(w, m);
+    if (a.scale != nullptr) {
+      to_f32<V, T>(sc, f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) m[j] *= 1.f + f[j];
+    }
+    put(s_mul, m);
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = 0.f;
+    if (a.shift != nullptr) to_f32<V, T>(sh, f);
+    put(s_shift, f);
+    if constexpr (TWO) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = 1.f;
+      if (a.gate != nullptr) to_f32<V, T>(g, f);
+      put(s_gate, f);
+    }
+  }
+  __syncthreads();
   for (; r < a.rows_per_batch; r += stride) {
     const long row = b * a.rows_per_batch + r;
     float y[N * V];
@@ -409,7 +452,7 @@ __global__ void __launch_bounds__(MULTI ? 32 * kMaxWarps : 128, MULTI ? 1 : 4)
         float f[V], g[V];
         to_f32<V, T>(x2[k], f);
         vector(s_gate, k, g);
-        if constexpr (V == 8) {
+        if constexpr (V > 1) {
 #pragma unroll
           for (int j = 0; j < V; j += 2)
             unpair(fma2(pair(g[j], g[j + 1]), pair(yk[j], yk[j + 1]), pair(f[j], f[j + 1])), yk[j], yk[j + 1]);
@@ -437,7 +480,7 @@ __global__ void __launch_bounds__(MULTI ? 32 * kMaxWarps : 128, MULTI ? 1 : 4)
       float mul[V], sh[V];
       vector(s_mul, k, mul);
       vector(s_shift, k, sh);
-      if constexpr (V == 8) {
+      if constexpr (V > 1) {
 #pragma unroll
         for (int j = 0; j < V; j += 2)
           unpair(fma2(mul2(pair(yk[j], yk[j + 1]), pair(rstd, rstd)), pair(mul[j], mul[j + 1]), pair(sh[j], sh[j + 1])),
@@ -514,14 +557,14 @@ __global__ void __launch_bounds__(512) quant_wide_kernel(const QuantArgs a) {
 }
 
 // q * s.  Rows of whole 16-byte groups: a thread turns 16 values of one row into
-// 32 (or 64) bytes; else neighbouring lanes take neighbouring values.
+// 32 (or 64) bytes; else neighbouring lanes take neighbouring values, V each.
 template <typename T>
 __global__ void __launch_bounds__(256) dequant_vec_kernel(const int8_t* __restrict__ q, long ldq,
                                                           const float* __restrict__ s, long groups, int per_row,
                                                           T* __restrict__ out) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= groups) return;
-  const long row = i / per_row;
+  const long row = groups <= 0x7FFFFFFFL ? (long)((unsigned)i / (unsigned)per_row) : i / per_row;
   const int e = (int)(i - row * per_row) * 16;
   const uint4 v = *reinterpret_cast<const uint4*>(q + row * ldq + e);
   const float sc = s[row];
@@ -534,28 +577,46 @@ __global__ void __launch_bounds__(256) dequant_vec_kernel(const int8_t* __restri
     store_v<8, T>(out + i * 16 + g * 8, f);
   }
 }
-template <typename T>
+template <typename T, int V>
 __global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* __restrict__ q, long ldq,
-                                                           const float* __restrict__ s, int D, T* __restrict__ out) {
-  const long row = blockIdx.x;
+                                                           const float* __restrict__ s, long R, int D,
+                                                           T* __restrict__ out) {
+  const long row = (long)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= R) return;
   const float sc = s[row];
-  for (int e0 = threadIdx.x; e0 < D; e0 += 4 * 256) {
-    int8_t v[4];
+  const int step = blockDim.x * V;
+  for (int e0 = threadIdx.x * V; e0 < D; e0 += 4 * step) {
+    uint16_t v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = e0 + j * 256 < D ? q[row * ldq + e0 + j * 256] : (int8_t)0;
+    for (int j = 0; j < 4; ++j) {
+      const int8_t* p = q + row * ldq + e0 + j * step;
+      v[j] = e0 + j * step >= D ? 0 : V == 2 ? *reinterpret_cast<const uint16_t*>(p) : (uint16_t)(uint8_t)*p;
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (e0 + j * 256 < D) from_f((float)v[j] * sc, out + row * D + e0 + j * 256);
+    for (int j = 0; j < 4; ++j) {
+      const float f[2] = {(float)(int8_t)v[j] * sc, (float)(int8_t)(v[j] >> 8) * sc};
+      if (e0 + j * step < D) store_v<V, T>(out + row * D + e0 + j * step, f);
+    }
   }
 }
 
 template <typename T>
 void launch_dequant(const int8_t* q, long ldq, const float* s, long R, int D, T* out, cudaStream_t stream) {
-  const bool vec = D % 16 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (R == 1 || ldq % 16 == 0);
-  const long blocks = vec ? (R * (D / 16) + 255) / 256 : R;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(q) | (R > 1 ? (uintptr_t)ldq : 0);
+  const bool vec = D % 16 == 0 && bits % 16 == 0;
+  const int V = D % 2 == 0 && bits % 2 == 0 ? 2 : 1;
+  // lanes a row, the rest of 256 threads over rows: the most that leave few of a lane's four slots idle
+  int lanes = 32, slots = 1 << 30;
+  for (int l = 256; l >= 32; l /= 2) {
+    const int n = (D + 4 * l * V - 1) / (4 * l * V) * 4 * l;
+    if (n < slots) { slots = n; lanes = l; }
+  }
+  const long blocks = vec ? (R * (D / 16) + 255) / 256 : (R + 256 / lanes - 1) / (256 / lanes);
   TORCH_CHECK(blocks <= 0x7FFFFFFFL, "dequant_rows: too many rows");
+  const dim3 block(lanes, 256 / lanes);
   if (vec) dequant_vec_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>(q, ldq, s, R * (D / 16), D / 16, out);
-  else dequant_rows_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>(q, ldq, s, D, out);
+  else if (V == 2) dequant_rows_kernel<T, 2><<<(unsigned)blocks, block, 0, stream>>>(q, ldq, s, R, D, out);
+  else dequant_rows_kernel<T, 1><<<(unsigned)blocks, block, 0, stream>>>(q, ldq, s, R, D, out);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   count_launch();
 }
@@ -585,103 +646,100 @@ void launch_sample(const QuantArgs& a, int warps, size_t smem, cudaStream_t stre
   kern<<<dim3((unsigned)blocks, (unsigned)samples), threads, smem, stream>>>(a, warps);
 }
 
-// The least warps that hold a row in N groups a thread with few idle slots.
+// The warps and groups a thread (at most `most`) with the fewest idle slots, of equals the fewest warps.
 struct RowShape {
   int warps, n;
 };
 RowShape fewest_warps(int groups, int most) {
   RowShape best = {0, 0};
-  double used = 0.0;
-  for (int w = 1; w <= kMaxWarps; ++w) {
-    const int n = (groups + 32 * w - 1) / (32 * w);
-    const double u = (double)groups / (32.0 * w * n);
-    if (n <= most && u > used * 1.02) { used = u; best = {w, n}; }
+  for (int n = most; n >= 1; --n) {
+    const int w = (groups + 32 * n - 1) / (32 * n);
+    if (w > kMaxWarps) break;
+    const int exact = (groups + 32 * w - 1) / (32 * w);
+    if (best.warps == 0 || 50 * w * exact < 49 * best.warps * best.n) best = {w, exact};
   }
   return best;
 }
 
-template <int MODE, typename T>
-void launch(const QuantArgs& a, bool vec, cudaStream_t stream) {
-  const int V = vec ? 8 : 1;
+// One of the instantiations of a kernel by V and N; `n` groups a thread at most.
+#define HARP_QUANT_BY_N(V_, n, CALL)            \
+  do {                                          \
+    if constexpr (V_ == 8) {                    \
+      switch (n) {                              \
+        case 1: CALL(8, 1); break;              \
+        case 2: CALL(8, 2); break;              \
+        case 3: CALL(8, 3); break;              \
+        case 4: CALL(8, 4); break;              \
+        default: CALL(8, 5); break;             \
+      }                                         \
+    } else if ((n) <= 4) {                      \
+      CALL(V_, 4);                              \
+    } else if ((n) <= 8) {                      \
+      CALL(V_, 8);                              \
+    } else {                                    \
+      CALL(V_, 16);                             \
+    }                                           \
+  } while (0)
+
+template <int MODE, typename T, int V>
+void launch(const QuantArgs& a, cudaStream_t stream) {
   const int groups = (a.D + V - 1) / V;
-  const RowShape many = fewest_warps(groups, vec ? 5 : 16);
-  const long samples = MODE >= kNorm ? a.R / a.rows_per_batch : 1;
-  bool done = false;
-  // Many rows: few warps a row, several groups a thread.
-  if (many.warps > 0 && a.R * many.warps > 8L * num_sms()) {
-    done = true;
+  const int lanes = V == 8 && groups <= 8 ? 8 : V == 8 && groups <= 16 ? 16 : 32;
+  RowShape many;
+  if (V == 8) {
+    many = fewest_warps(groups, 5);
+  } else {
+    // one warp for up to 16 groups a lane (a 333 wide bf16 row: 6.1 us, 8.5 on two warps), else 8
+    // groups a lane (1155 wide: 69 us with a residual, 118 with 16)
+    const int most = groups <= 512 ? 16 : groups <= 256 * kMaxWarps ? 8 : 16;
+    const int w = (groups + 32 * most - 1) / (32 * most);
+    many = {w <= kMaxWarps ? w : 0, (groups + 32 * w - 1) / (32 * w)};
+  }
+  if (many.warps == 0) {
+    TORCH_CHECK(a.R <= 0x7FFFFFFFL, "harp quant: too many rows");
+    quant_wide_kernel<MODE, T><<<(unsigned)a.R, 512, 0, stream>>>(a);
+  } else if (a.R * many.warps <= 8L * num_sms()) {
+    // Few rows: latency counts, so as many warps as the row has groups for.
+    auto with = [&](int n) { return std::max(1, (groups + 32 * n - 1) / (32 * n)); };
+    const int n = (groups + 32 * kMaxWarps - 1) / (32 * kMaxWarps);
+#define HARP_FEW(V_, N_) launch_few<MODE, T, V_, N_>(a, N_ == 1 ? lanes : 32, with(N_), stream)
+    HARP_QUANT_BY_N(V, n, HARP_FEW);
+#undef HARP_FEW
+  } else {
+    bool by_sample = false;
     if constexpr (MODE >= kNorm) {
       const size_t smem = (size_t)groups * V * 4 * (MODE == kNormRes ? 3 : 2);
-      if (smem <= kVecSmem && samples <= 65535 && a.rows_per_batch >= 8) {
-#define HARP_SAMPLE(V_, N_)                                                                   \
-  (many.warps == 1 ? launch_sample<MODE, T, V_, N_, false>(a, many.warps, smem, stream)       \
+      by_sample = smem <= kVecSmem && a.R / a.rows_per_batch <= 65535 && a.rows_per_batch >= 8;
+      if (by_sample) {
+#define HARP_SAMPLE(V_, N_)                                                                 \
+  (many.warps == 1 ? launch_sample<MODE, T, V_, N_, false>(a, many.warps, smem, stream)     \
                    : launch_sample<MODE, T, V_, N_, true>(a, many.warps, smem, stream))
-        if (vec) {
-          switch (many.n) {
-            case 1: HARP_SAMPLE(8, 1); break;
-            case 2: HARP_SAMPLE(8, 2); break;
-            case 3: HARP_SAMPLE(8, 3); break;
-            case 4: HARP_SAMPLE(8, 4); break;
-            default: HARP_SAMPLE(8, 5); break;
-          }
-        } else if (many.n <= 4) {
-          HARP_SAMPLE(1, 4);
-        } else if (many.n <= 8) {
-          HARP_SAMPLE(1, 8);
-        } else {
-          HARP_SAMPLE(1, 16);
-        }
+        HARP_QUANT_BY_N(V, many.n, HARP_SAMPLE);
 #undef HARP_SAMPLE
-      } else {
-        done = false;
       }
-    } else if (vec) {
-      const int lanes = groups <= 8 ? 8 : groups <= 16 ? 16 : 32;
-      switch (many.n) {
-        case 1: launch_few<MODE, T, 8, 1>(a, lanes, many.warps, stream); break;
-        case 2: launch_few<MODE, T, 8, 2>(a, 32, many.warps, stream); break;
-        case 3: launch_few<MODE, T, 8, 3>(a, 32, many.warps, stream); break;
-        case 4: launch_few<MODE, T, 8, 4>(a, 32, many.warps, stream); break;
-        default: launch_few<MODE, T, 8, 5>(a, 32, many.warps, stream); break;
-      }
-    } else if (many.n <= 4) {
-      launch_few<MODE, T, 1, 4>(a, 32, many.warps, stream);
-    } else if (many.n <= 8) {
-      launch_few<MODE, T, 1, 8>(a, 32, many.warps, stream);
-    } else {
-      launch_few<MODE, T, 1, 16>(a, 32, many.warps, stream);
     }
-  }
-  if (!done) {
-    // Few rows: latency counts, so as many warps as the row has groups for.
-    const int n = (groups + 32 * kMaxWarps - 1) / (32 * kMaxWarps);
-    const int lanes = vec && groups <= 8 ? 8 : vec && groups <= 16 ? 16 : 32;
-    auto warps = [&](int per_thread) { return std::max(1, (groups + 32 * per_thread - 1) / (32 * per_thread)); };
-    if (vec && n == 1) {
-      launch_few<MODE, T, 8, 1>(a, lanes, warps(1), stream);
-    } else if (vec && n == 2) {
-      launch_few<MODE, T, 8, 2>(a, 32, warps(2), stream);
-    } else if (vec && n <= 5) {
-      launch_few<MODE, T, 8, 5>(a, 32, warps(5), stream);
-    } else if (!vec && n <= 4) {
-      launch_few<MODE, T, 1, 4>(a, 32, warps(4), stream);
-    } else if (!vec && n <= 8) {
-      launch_few<MODE, T, 1, 8>(a, 32, warps(8), stream);
-    } else if (!vec && n <= 16) {
-      launch_few<MODE, T, 1, 16>(a, 32, warps(16), stream);
-    } else {
-      TORCH_CHECK(a.R <= 0x7FFFFFFFL, "harp quant: too many rows");
-      quant_wide_kernel<MODE, T><<<(unsigned)a.R, 512, 0, stream>>>(a);
+    if (!by_sample) {
+#define HARP_MANY(V_, N_) launch_few<MODE, T, V_, N_>(a, N_ == 1 ? lanes : 32, many.warps, stream)
+      HARP_QUANT_BY_N(V, many.n, HARP_MANY);
+#undef HARP_MANY
     }
   }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   count_launch();
 }
 
+// width: 8, 2 or 1 values an access
 template <int MODE>
-void launch_mode(const QuantArgs& a, at::ScalarType t, bool vec, cudaStream_t stream) {
-  if (t == at::kBFloat16) launch<MODE, bf16>(a, vec, stream);
-  else launch<MODE, float>(a, vec, stream);
+void launch_mode(const QuantArgs& a, at::ScalarType t, int width, cudaStream_t stream) {
+  if (t == at::kBFloat16) {
+    if (width == 8) launch<MODE, bf16, 8>(a, stream);
+    else if (width == 2) launch<MODE, bf16, 2>(a, stream);
+    else launch<MODE, bf16, 1>(a, stream);
+  } else {
+    if (width == 8) launch<MODE, float, 8>(a, stream);
+    else if (width == 2) launch<MODE, float, 2>(a, stream);
+    else launch<MODE, float, 1>(a, stream);
+  }
 }
 
 // Numbers in messages go through std::to_string: with a statically linked libstdc++ (as some
@@ -698,18 +756,22 @@ void check_rows(const at::Tensor& x, const char* op, const char* name) {
   TORCH_CHECK(x.stride(1) == 1 || x.size(1) == 1, op, ": ", name, " needs a unit inner stride");
 }
 
-// 16-byte accesses are possible on every row of t.
-bool vec_ok(const at::Tensor& t) {
-  return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 &&
-         (t.dim() < 2 || t.size(0) <= 1 || (t.stride(0) * t.element_size()) % 16 == 0);
+// The bits that keep a tensor's rows from alignment: its address and row stride in bytes.
+uintptr_t low_bits(const at::Tensor& t) {
+  uintptr_t b = reinterpret_cast<uintptr_t>(t.data_ptr());
+  if (t.dim() == 2 && t.size(0) > 1) b |= (uintptr_t)(t.stride(0) * t.element_size());
+  return b;
+}
+int width_of(uintptr_t bits, int64_t D, int esize) {
+  return D % 8 == 0 && bits % 16 == 0 ? 8 : D % 2 == 0 && bits % (2 * esize) == 0 ? 2 : 1;
 }
 
 // q [R, D] with rows on 16-byte boundaries (what TMA can address), s [R]
 std::tuple<at::Tensor, at::Tensor> new_rows8(const at::Tensor& x, int64_t R, int64_t D) {
   const int64_t ld = (D + 15) / 16 * 16;
-  at::Tensor q(at::detail::empty_cuda({R, ld}, at::kChar, x.device(), c10::nullopt));
+  at::Tensor q(at::detail::empty_strided_cuda({R, D}, {ld, 1}, at::kChar, x.device()));
   at::Tensor s(at::detail::empty_cuda({R}, at::kFloat, x.device(), c10::nullopt));
-  return {ld == D ? q : q.narrow(1, 0, D), s};
+  return {q, s};
 }
 
 void set_out(QuantArgs& a, const at::Tensor& q, const at::Tensor& s) {
@@ -728,10 +790,10 @@ std::tuple<at::Tensor, at::Tensor> rows_or_swiglu(const at::Tensor& x, int64_t D
   set_out(a, q, s);
   a.x = x.data_ptr();
   a.ldx = x.stride(0);
-  const bool vec = D % 8 == 0 && vec_ok(x);
+  const int width = width_of(low_bits(x), D, (int)x.element_size());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  if (swiglu) launch_mode<kSwiglu>(a, x.scalar_type(), vec, stream);
-  else launch_mode<kRows>(a, x.scalar_type(), vec, stream);
+  if (swiglu) launch_mode<kSwiglu>(a, x.scalar_type(), width, stream);
+  else launch_mode<kRows>(a, x.scalar_type(), width, stream);
   return {q, s};
 }
 
@@ -761,7 +823,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rmsnorm_mod_quant(
               num(R), " rows are not whole samples of ", num(rows_per_batch));
   const at::cuda::CUDAGuard guard(x.device());
   QuantArgs a = {};
-  bool vec = D % 8 == 0 && vec_ok(x);
+  uintptr_t bits = low_bits(x);
   a.x = x.data_ptr();
   a.ldx = x.stride(0);
   a.eps = (float)eps;
@@ -771,7 +833,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rmsnorm_mod_quant(
                     w->size(0) == D && (D == 1 || w->stride(0) == 1),
                 op, ": w must be a dense vector of ", num(D), " values of x's type on x's device");
     a.w = w->data_ptr();
-    vec = vec && vec_ok(*w);
+    bits |= low_bits(*w);
   }
   auto vectors = [&](const c10::optional<at::Tensor>& v, const char* name, const void*& p, long& ld) {
     if (!v.has_value()) return;
@@ -781,7 +843,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rmsnorm_mod_quant(
                 "] of x's type on x's device with a unit inner stride");
     p = v->data_ptr();
     ld = v->stride(0);
-    vec = vec && vec_ok(*v);
+    bits |= low_bits(*v);
   };
   vectors(scale, "scale", a.scale, a.ld_scale);
   vectors(shift, "shift", a.shift, a.ld_shift);
@@ -797,14 +859,15 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rmsnorm_mod_quant(
     h = at::Tensor(at::detail::empty_cuda({R, D}, x.scalar_type(), x.device(), c10::nullopt));
     a.h = h.data_ptr();
     a.ldh = D;
-    vec = vec && vec_ok(*residual);
+    bits |= low_bits(*residual);
   }
   auto [q, s] = new_rows8(x, R, D);
   if (R == 0) return {q, s, h};
   set_out(a, q, s);
+  const int width = width_of(bits, D, (int)x.element_size());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  if (residual.has_value()) launch_mode<kNormRes>(a, x.scalar_type(), vec, stream);
-  else launch_mode<kNorm>(a, x.scalar_type(), vec, stream);
+  if (residual.has_value()) launch_mode<kNormRes>(a, x.scalar_type(), width, stream);
+  else launch_mode<kNorm>(a, x.scalar_type(), width, stream);
   return {q, s, h};
 }
 

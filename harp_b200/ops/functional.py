@@ -31,7 +31,8 @@ EPI_GATED_RESIDUAL_SAVE = 5
 
 def _cuda(t: torch.Tensor) -> bool:
     if t.is_cuda:
-        _native.require()
+        if not _native._loaded:
+            _native.require()
         return True
     return False
 

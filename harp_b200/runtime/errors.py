@@ -28,7 +28,9 @@ class HarpDeviceError(RuntimeError):
 
 
 def word(device: torch.device) -> torch.Tensor:
-    idx = device.index if device.index is not None else torch.cuda.current_device()
+    idx = device.index
+    if idx is None:
+        idx = torch.cuda.current_device()
     w = _words.get(idx)
     if w is None:
         with _lock:
