@@ -15,6 +15,7 @@
 //                 weights' bytes and the latency count
 //   gemm_s8_simt  CUDA cores, for operands TMA cannot address
 #include "common.cuh"
+#include "dependent_launch.cuh"
 #include "gemm_common.cuh"
 #include "gemm_sm100.h"
 
@@ -210,6 +211,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   cluster_sync_all();  // both CTAs' barriers exist and the paired TMEM is allocated
+  dependency_release();
+  dependency_wait();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
@@ -507,6 +510,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  dependency_release();
+  dependency_wait();
   const uint32_t tmem_base = *tmem_slot;
   bool have = false;  // epilogue warps: this CTA's sums are in tensor memory
 
@@ -614,6 +619,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 __global__ void __launch_bounds__(256) gemm_s8_simt(const S8Args a) {
   __shared__ int As[32][33];
   __shared__ int Bs[32][33];
+  dependency_release();
+  dependency_wait();
   const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;  // 32 x 8 threads
   const int m0 = blockIdx.y * 32, n0 = blockIdx.x * 32;
   int acc[4] = {0, 0, 0, 0};
@@ -664,29 +671,32 @@ CUtensorMap make_map_s8(const int8_t* base, long rows, long cols, long ld, int b
   return make_map(base, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, cols, ld, box_rows);
 }
 
+// Clusters of `cluster` blocks that the device keeps resident at once (GPC shapes leave
+// SMs over), with the kernel set up for its shared memory.
+template <typename... P>
+int resident_clusters(void (*kern)(P...), int cluster, int smem) {
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(num_sms() / cluster * cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  C10_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+  return std::max(1, n);
+}
+
 template <int BN, typename OUT>
 void launch_pair(const S8Args& a, bool c_tma, cudaStream_t stream) {
   using C_ = PairCfg<BN>;
   auto kern = gemm_s8_pair<BN, OUT>;
-  static int max_clusters = 0;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C_::SMEM_BYTES;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (max_clusters == 0) {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM_BYTES));
-    cfg.gridDim = dim3(2 * (num_sms() / 2));
-    int n = 0;
-    C10_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
-    max_clusters = std::max(1, n);
-  }
+  static const int max_clusters = resident_clusters(kern, 2, C_::SMEM_BYTES);
   const CUtensorMap ta = make_map_s8(a.A, a.M, a.K, a.lda, 128), tb = make_map_s8(a.B, a.N, a.K, a.ldb, BN / 2);
   CUtensorMap tc = ta;
   if (c_tma)
@@ -694,8 +704,8 @@ void launch_pair(const S8Args& a, bool c_tma, cudaStream_t stream) {
                   sizeof(OUT), a.M, a.N, a.ldc * (long)sizeof(OUT), 32);
   const long tiles = (long)((a.M + 255) / 256) * ((a.N + BN - 1) / BN);
   TORCH_CHECK(tiles <= 0x3FFFFFFF, "harp gemm_s8: too many tiles");
-  cfg.gridDim = dim3(2 * (unsigned)std::min<long>(tiles, max_clusters));
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, tc, a, c_tma ? 1 : 0));
+  launch_dependent(kern, dim3(2 * (unsigned)std::min<long>(tiles, max_clusters)), dim3(kThreads), C_::SMEM_BYTES, stream,
+                   2, ta, tb, tc, a, c_tma ? 1 : 0);
   count_launch();
 }
 
@@ -703,27 +713,13 @@ template <int NT, typename OUT>
 void launch_rows(const S8Args& a, int splits, cudaStream_t stream) {
   using C_ = RowsCfg<NT>;
   auto kern = gemm_s8_rows<NT, OUT>;
-  static bool configured = false;
-  if (!configured) {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM_BYTES));
-    configured = true;
-  }
+  static const cudaError_t configured =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM_BYTES);
+  C10_CUDA_CHECK(configured);
   const CUtensorMap tw = make_map_s8(a.B, a.N, a.K, a.ldb, 128), tx = make_map_s8(a.A, a.M, a.K, a.lda, NT);
   const long ctas = (long)((a.N + 127) / 128) * ((a.M + NT - 1) / NT) * splits;
   TORCH_CHECK(ctas <= 0x7FFFFFFF, "harp gemm_s8: too many tiles");
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)splits;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C_::SMEM_BYTES;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = splits > 1 ? 1 : 0;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tw, tx, a, splits));
+  launch_dependent(kern, dim3((unsigned)ctas), dim3(kThreads), C_::SMEM_BYTES, stream, splits, tw, tx, a, splits);
   count_launch();
 }
 
@@ -734,23 +730,7 @@ long cluster_slots(int splits) {
   if (splits == 1) return num_sms();
   long n = slots[splits].load(std::memory_order_relaxed);
   if (n == 0) {
-    using C_ = RowsCfg<16>;
-    auto kern = gemm_s8_rows<16, bf16>;
-    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM_BYTES));
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)splits;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(num_sms() / splits * splits));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = C_::SMEM_BYTES;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int clusters = 0;
-    C10_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg));
-    n = std::max(1, clusters * splits);
+    n = (long)splits * resident_clusters(gemm_s8_rows<16, bf16>, splits, RowsCfg<16>::SMEM_BYTES);
     slots[splits].store(n, std::memory_order_relaxed);
   }
   return n;
@@ -889,8 +869,7 @@ void gemm_s8_out(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B,
   }
   dim3 grid((unsigned)((N + 31) / 32), (unsigned)((M + 31) / 32));
   TORCH_CHECK(grid.y <= 65535, "harp gemm_s8: too many rows for the CUDA-core path");
-  gemm_s8_simt<<<grid, 256, 0, stream>>>(a);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  launch_dependent(gemm_s8_simt, grid, dim3(256), 0, stream, 1, a);
   count_launch();
 }
 

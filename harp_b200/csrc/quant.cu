@@ -19,6 +19,7 @@
 // Bound by memory: each value is read once and held in registers between the
 // row's reductions and the rounding.
 #include "common.cuh"
+#include "dependent_launch.cuh"
 #include "gemm_sm100.h"
 
 #include <ATen/ATen.h>
@@ -272,6 +273,8 @@ template <int MODE, typename T, int V, int N>
 __global__ void __launch_bounds__(32 * kMaxWarps) quant_rows_kernel(const QuantArgs a, int lanes, int warps) {
   constexpr bool NORM = MODE >= kNorm, TWO = MODE == kSwiglu || MODE == kNormRes;
   __shared__ float red[2][32];
+  dependency_release();
+  dependency_wait();
   const int per_row = lanes * warps;
   const int t = warps == 1 ? threadIdx.x % lanes : threadIdx.x;
   const long at = warps == 1 ? (long)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes : (long)blockIdx.x;
@@ -368,6 +371,8 @@ __global__ void __launch_bounds__(MULTI ? 32 * kMaxWarps : 128, MULTI ? 1 : MODE
   constexpr int H = V == 8 ? 4 : V;  // a vector lies in V / H planes, so that wide reads meet no bank twice
   extern __shared__ __align__(16) float vec[];
   __shared__ float red[2][32];
+  dependency_release();
+  dependency_wait();
   const int slots = (a.D + V - 1) / V;
   float* const s_mul = vec;  // each [V / H][slots][H]
   float* const s_shift = s_mul + slots * V;
@@ -531,6 +536,8 @@ __device__ __forceinline__ float wide_y(const QuantArgs& a, long row, long b, in
 template <int MODE, typename T>
 __global__ void __launch_bounds__(512) quant_wide_kernel(const QuantArgs a) {
   __shared__ float red[2][32];
+  dependency_release();
+  dependency_wait();
   const int warps = blockDim.x / 32;
   const long row = blockIdx.x;
   const long b = MODE >= kNorm ? row / a.rows_per_batch : 0;
@@ -562,6 +569,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) dequant_vec_kernel(const int8_t* __restrict__ q, long ldq,
                                                           const float* __restrict__ s, long groups, int per_row,
                                                           T* __restrict__ out) {
+  dependency_release();
+  dependency_wait();
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= groups) return;
   const long row = groups <= 0x7FFFFFFFL ? (long)((unsigned)i / (unsigned)per_row) : i / per_row;
@@ -581,6 +590,8 @@ template <typename T, int V>
 __global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* __restrict__ q, long ldq,
                                                            const float* __restrict__ s, long R, int D,
                                                            T* __restrict__ out) {
+  dependency_release();
+  dependency_wait();
   const long row = (long)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= R) return;
   const float sc = s[row];
@@ -614,10 +625,9 @@ void launch_dequant(const int8_t* q, long ldq, const float* s, long R, int D, T*
   const long blocks = vec ? (R * (D / 16) + 255) / 256 : (R + 256 / lanes - 1) / (256 / lanes);
   TORCH_CHECK(blocks <= 0x7FFFFFFFL, "dequant_rows: too many rows");
   const dim3 block(lanes, 256 / lanes);
-  if (vec) dequant_vec_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>(q, ldq, s, R * (D / 16), D / 16, out);
-  else if (V == 2) dequant_rows_kernel<T, 2><<<(unsigned)blocks, block, 0, stream>>>(q, ldq, s, R, D, out);
-  else dequant_rows_kernel<T, 1><<<(unsigned)blocks, block, 0, stream>>>(q, ldq, s, R, D, out);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (vec) launch_dependent(dequant_vec_kernel<T>, (unsigned)blocks, 256, 0, stream, 1, q, ldq, s, R * (D / 16), D / 16, out);
+  else if (V == 2) launch_dependent(dequant_rows_kernel<T, 2>, (unsigned)blocks, block, 0, stream, 1, q, ldq, s, R, D, out);
+  else launch_dependent(dequant_rows_kernel<T, 1>, (unsigned)blocks, block, 0, stream, 1, q, ldq, s, R, D, out);
   count_launch();
 }
 
@@ -627,7 +637,7 @@ void launch_few(const QuantArgs& a, int lanes, int warps, cudaStream_t stream) {
   const int per_block = warps == 1 ? threads / lanes : 1;
   const long blocks = (a.R + per_block - 1) / per_block;
   TORCH_CHECK(blocks <= 0x7FFFFFFFL, "harp quant: too many rows");
-  quant_rows_kernel<MODE, T, V, N><<<(unsigned)blocks, threads, 0, stream>>>(a, lanes, warps);
+  launch_dependent(quant_rows_kernel<MODE, T, V, N>, (unsigned)blocks, threads, 0, stream, 1, a, lanes, warps);
 }
 
 template <int MODE, typename T, int V, int N, bool MULTI>
@@ -643,7 +653,7 @@ void launch_sample(const QuantArgs& a, int warps, size_t smem, cudaStream_t stre
   const long samples = a.R / a.rows_per_batch;
   const long most = (a.rows_per_batch + per_block - 1) / per_block;
   const long blocks = std::max<long>(1, std::min<long>(most, (long)std::max(1, n) * num_sms() / samples));
-  kern<<<dim3((unsigned)blocks, (unsigned)samples), threads, smem, stream>>>(a, warps);
+  launch_dependent(kern, dim3((unsigned)blocks, (unsigned)samples), threads, smem, stream, 1, a, warps);
 }
 
 // The warps and groups a thread (at most `most`) with the fewest idle slots, of equals the fewest warps.
@@ -697,7 +707,7 @@ void launch(const QuantArgs& a, cudaStream_t stream) {
   }
   if (many.warps == 0) {
     TORCH_CHECK(a.R <= 0x7FFFFFFFL, "harp quant: too many rows");
-    quant_wide_kernel<MODE, T><<<(unsigned)a.R, 512, 0, stream>>>(a);
+    launch_dependent(quant_wide_kernel<MODE, T>, (unsigned)a.R, 512, 0, stream, 1, a);
   } else if (a.R * many.warps <= 8L * num_sms()) {
     // Few rows: latency counts, so as many warps as the row has groups for.
     auto with = [&](int n) { return std::max(1, (groups + 32 * n - 1) / (32 * n)); };
@@ -724,7 +734,6 @@ void launch(const QuantArgs& a, cudaStream_t stream) {
 #undef HARP_MANY
     }
   }
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
   count_launch();
 }
 

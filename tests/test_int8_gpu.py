@@ -389,3 +389,42 @@ def test_sampling_with_the_int8_dit():
     ref = batch_image_inference(m, **kw)["images"].float()
     out = batch_image_inference(m.int8(), **kw)["images"].float()
     assert torch.isfinite(out).all() and ((out - ref).norm() / ref.norm()).item() < 6e-2
+
+
+def test_dependent_launches_are_ordered():
+    """The kernels may start before the one ahead of them on the stream has finished; what they read and
+    write has to be as if they had not: a chain through the same buffers, against one with a wait after
+    every step.  Exact integer sums make both bit-identical."""
+    g = torch.Generator().manual_seed(7)
+    for M, N in ((3, 1152), (288, 1152), (1100, 1152), (5000, 1152)):
+        x0 = torch.randn(M, N, generator=g).bfloat16().cuda()
+        w = [Fn.quant_rows(torch.randn(N, N, generator=g).cuda() * N ** -0.5) for _ in range(3)]
+
+        def chain(wait):
+            x, h = x0.clone(), x0.clone()
+            out = torch.empty_like(x)
+            for i in range(30):
+                q, s, h = Fn.rmsnorm_mod_quant(x, None, None, None, M, 1e-6, residual=h)
+                wait()
+                Fn.gemm_s8(q, s, *w[i % 3], out=out)
+                wait()
+                q, s = Fn.quant_rows(out)
+                wait()
+                Fn.gemm_s8(q, s, *w[(i + 1) % 3], out=out)  # over the rows just quantised
+                wait()
+                x = out if i % 2 else out.clone()  # now and then a kernel launched in the ordinary way
+                wait()
+            return x.clone(), h
+
+        a = chain(torch.cuda.synchronize)
+        b = chain(lambda: None)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c = chain(lambda: None)
+        for t in c:
+            t.zero_()
+        graph.replay()
+        graph.replay()
+        assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
+    errors.check(x0.device)
