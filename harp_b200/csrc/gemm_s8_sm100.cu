@@ -138,6 +138,10 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
   return p != 0;
 }
+// A wait of the whole warp with one answer (lanes that ran out of time a moment apart must not part ways).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int site) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, err, site)) != 0;
+}
 // Arrive on another CTA's barrier without ordering earlier stores: what the
 // barrier hands over is tensor memory, which the tcgen05 fences order.  (With
 // release.cluster the arrive waits for the stores of the epilogue: 1700 clocks a
@@ -263,14 +267,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = pair; t < num_tiles && ok; t += npairs, ++local) {
         const int acc = local & 1;
         const uint32_t acc_phase = (local >> 1) & 1;
-        if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1, err, 62)) { ok = false; break; }
+        if (!warp_wait(&tempty_bar[acc], acc_phase ^ 1, err, 62)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
         int mt, nt;
         pair_tile(t, num_m, num_n, args.N % BN != 0, mt, nt);
         const uint32_t idesc = make_idesc_s8(256, 2 * min(BN / 2, ((args.N - nt * BN + 31) / 32) * 16));
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&full_bar[stage], phase, err, 63)) { ok = false; break; }
+          if (!warp_wait(&full_bar[stage], phase, err, 63)) { ok = false; break; }
           tc_fence_after();
           const uint64_t ad = a0 + (uint64_t)(stage * (C_::A_BYTES >> 4));
           const uint64_t bd = b0 + (uint64_t)(stage * (C_::B_BYTES >> 4));
@@ -341,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       epilogue_barrier();
       if (t + npairs < num_tiles) fetch(t + npairs);
-      ok = ok && mbar_wait(&tfull_bar[acc], acc_phase, err, 64);
+      ok = ok && warp_wait(&tfull_bar[acc], acc_phase, err, 64);
       if (!ok) continue;
       tc_fence_after();
       const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
@@ -514,6 +518,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   dependency_wait();
   const uint32_t tmem_base = *tmem_slot;
   bool have = false;  // epilogue warps: this CTA's sums are in tensor memory
+  const int n = n0 + lane * 4;  // a lane's channels in the last step
+  float sb[4] = {}, bias[4] = {};
 
   if (warp == 0) {
     if (lane == 0) {
@@ -540,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int stage = 0;
     uint32_t phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (!mbar_wait(&full_bar[stage], phase, err, 72)) break;
+      if (!warp_wait(&full_bar[stage], phase, err, 72)) break;
       tc_fence_after();
       if (issue) {
 #pragma unroll
@@ -560,7 +566,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3;
     const int ch = quarter * 32 + lane;
     for (int j = threadIdx.x - 64; j < NT; j += 128) tok_scale[j] = m0 + j < args.M ? args.sa[m0 + j] : 0.f;
-    have = mbar_wait(done_bar, 0, err, 73);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (n + i < args.N) {
+        sb[i] = args.sb[n + i];
+        bias[i] = bias_at(args, n + i);
+      }
+    }
+    have = warp_wait(done_bar, 0, err, 73);
     tc_fence_after();
     const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16);
     constexpr int W = NT < 32 ? NT : 32;  // tokens a step
@@ -582,13 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   else __syncthreads();
   if (warp >= 2 && have) {
     // a warp takes every fourth token of this rank's share, a lane four channels of it
-    const int t0 = rank * NT / splits, t1 = (rank + 1) * NT / splits, n = n0 + lane * 4;
-    float sb[4], bias[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sb[i] = n + i < args.N ? args.sb[n + i] : 0.f;
-      bias[i] = n + i < args.N ? bias_at(args, n + i) : 0.f;
-    }
+    const int t0 = rank * NT / splits, t1 = (rank + 1) * NT / splits;
     const uint32_t mine = smem_u32(smem) + (uint32_t)lane * 16;
 #pragma unroll 4
     for (int j = t0 + warp - 2; j < t1; j += 4) {

@@ -273,7 +273,6 @@ template <int MODE, typename T, int V, int N>
 __global__ void __launch_bounds__(32 * kMaxWarps) quant_rows_kernel(const QuantArgs a, int lanes, int warps) {
   constexpr bool NORM = MODE >= kNorm, TWO = MODE == kSwiglu || MODE == kNormRes;
   __shared__ float red[2][32];
-  dependency_release();
   dependency_wait();
   const int per_row = lanes * warps;
   const int t = warps == 1 ? threadIdx.x % lanes : threadIdx.x;
@@ -371,7 +370,6 @@ __global__ void __launch_bounds__(MULTI ? 32 * kMaxWarps : 128, MULTI ? 1 : MODE
   constexpr int H = V == 8 ? 4 : V;  // a vector lies in V / H planes, so that wide reads meet no bank twice
   extern __shared__ __align__(16) float vec[];
   __shared__ float red[2][32];
-  dependency_release();
   dependency_wait();
   const int slots = (a.D + V - 1) / V;
   float* const s_mul = vec;  // each [V / H][slots][H]
@@ -536,7 +534,6 @@ __device__ __forceinline__ float wide_y(const QuantArgs& a, long row, long b, in
 template <int MODE, typename T>
 __global__ void __launch_bounds__(512) quant_wide_kernel(const QuantArgs a) {
   __shared__ float red[2][32];
-  dependency_release();
   dependency_wait();
   const int warps = blockDim.x / 32;
   const long row = blockIdx.x;
@@ -569,7 +566,6 @@ template <typename T>
 __global__ void __launch_bounds__(256) dequant_vec_kernel(const int8_t* __restrict__ q, long ldq,
                                                           const float* __restrict__ s, long groups, int per_row,
                                                           T* __restrict__ out) {
-  dependency_release();
   dependency_wait();
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= groups) return;
@@ -590,7 +586,6 @@ template <typename T, int V>
 __global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* __restrict__ q, long ldq,
                                                            const float* __restrict__ s, long R, int D,
                                                            T* __restrict__ out) {
-  dependency_release();
   dependency_wait();
   const long row = (long)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= R) return;
