@@ -8,12 +8,18 @@
 //
 // Three kernels:
 //   gemm_s8_pair  CTA pairs (cta_group::2), persistent over 256 x BN tiles: many
-//                 tokens and many channels; bound by the tensor pipe
+//                 tokens and many channels.  Bound by the tensor pipe and, in a
+//                 long run, by power: 17408 x 9216 x 1152 in 138 to 165 us (2.7 to
+//                 2.2 PFLOP/s), 17408 x 1152 x 4608 in 69 to 82 us; run for a
+//                 second the GPU sits at its 1000 W and 1.37 GHz (zeros for operands:
+//                 119 us at 1.97 GHz)
 //   gemm_s8_rows  128 channels x up to 256 tokens a CTA, the K loop split over a
 //                 cluster that adds its integer sums through distributed shared
-//                 memory: few tokens (down to one) or few channels, where the
-//                 weights' bytes and the latency count
-//   gemm_s8_simt  CUDA cores, for operands TMA cannot address
+//                 memory: few tokens (down to one) or few channels.  Bound by
+//                 latency: 4 x 6912 x 1152 4.5 to 5.9 us, 4 x 1152 x 4608 4.6 us back to
+//                 back, of which the weights' bytes are 1.2 and 0.8 us
+//   gemm_s8_simt  CUDA cores, for operands TMA cannot address (1061 x 1003 x 1155 with
+//                 odd row strides: 259 us, against 12 to 16 in the pair kernel)
 #include "common.cuh"
 #include "dependent_launch.cuh"
 #include "gemm_common.cuh"
@@ -108,12 +114,15 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 // each CTA stages its own 128 rows of A and BN/2 rows of B, the leader issues
 // M = 256 MMAs, two accumulators let the epilogue of one tile run under the MMAs
 // of the next.  A stage is 256 deep in K (two 128-byte swizzle atoms a row), the
-// same bytes as the bf16 kernel's 128, at twice the arithmetic.
+// same bytes as the bf16 kernel's 128, at twice the arithmetic.  (Stages of 128 and
+// a commit for four MMAs instead of eight: 17408 x 1152 x 4608 in 101 us, not 83.)
 //
 // Epilogue: each warp scales its 32 rows 128 bytes at a time, lays them out in
 // shared memory and one lane stores the block with TMA (whole 128-byte lines;
 // out of range rows and columns are dropped by the map).  A C that TMA cannot
-// address is written from the same buffer, a row of the block at a time.
+// address is written from the same buffer, a row of the block at a time.  Stored
+// straight from registers, 32 bytes a lane, 17408 x 9216 x 1152 took 187 us, not 154;
+// eight epilogue warps instead of four changed nothing (190 and 187 at that time).
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 192;
 constexpr int kStageK = 256;
@@ -255,7 +264,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (leader CTA) ----------------
-    // The whole warp keeps the loop's state, so that it stays in uniform registers; one lane issues.
+    // The whole warp keeps the loop's state, so that it stays in uniform registers; one lane issues
+    // (a lone thread moved each descriptor to uniform registers for each MMA: 169 us, not 156).
     if (rank == 0) {
       const bool issue = elect_one();
       const uint64_t a0 = make_sdesc(smem_u32(smem_a), 16, 1024, kLayoutSw128);

@@ -17,7 +17,13 @@
 // NaN, as it is in bf16.
 //
 // Bound by memory: each value is read once and held in registers between the
-// row's reductions and the rounding.
+// row's reductions and the rounding.  Measured on one B200 (inputs and outputs over
+// the kernel's time; 6.5 TB/s is a copy), bf16: quant_rows of 17408 x 1152 10.3 us
+// (5.8 TB/s), swiglu_quant of 17408 x 4608 66 us (6.0), rmsnorm_mod_quant of 17408 x
+// 1152 with residual, gate and modulation 20.4 us (6.9, part of it from L2), dequant_rows
+// of 17408 x 1152 10.9 us (5.5); one to a few hundred rows take 2 to 3 us, launch included.
+// Widths that are not multiples of 8 read 2 or 1 values at a time: 17408 x 1154 22 us,
+// 17408 x 1155 31 us (bound by instructions).
 #include "common.cuh"
 #include "dependent_launch.cuh"
 #include "gemm_sm100.h"

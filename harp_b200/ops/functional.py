@@ -411,6 +411,14 @@ def _rows8(y: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return q, torch.where(bad, torch.full_like(s, float("nan")), s)
 
 
+def _is_f32(dtype: torch.dtype, op: str) -> bool:
+    if dtype is torch.bfloat16:
+        return False
+    if dtype is torch.float32:
+        return True
+    raise RuntimeError(f"{op}: bf16 or fp32 output, not {dtype}")
+
+
 def _check_rows(x: torch.Tensor, op: str) -> None:
     if x.dtype not in (torch.bfloat16, torch.float32) or x.dim() != 2 or x.shape[1] < 1:
         raise RuntimeError(f"{op}: a 2-D bf16 or fp32 tensor with at least one column is required")
@@ -431,10 +439,9 @@ def quant_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 def dequant_rows(q: torch.Tensor, s: torch.Tensor, dtype=torch.bfloat16) -> torch.Tensor:
     """``q * s`` of :func:`quant_rows` in bf16 or fp32."""
-    if dtype not in (torch.bfloat16, torch.float32):
-        raise RuntimeError(f"dequant_rows: bf16 or fp32 output, not {dtype}")
+    f32 = _is_f32(dtype, "dequant_rows")
     if _cuda(q):
-        return torch.ops.harp.dequant_rows(q, s, dtype == torch.float32)
+        return torch.ops.harp.dequant_rows(q, s, f32)
     return (q.float() * s[:, None]).to(dtype)
 
 
@@ -494,11 +501,9 @@ def gemm_s8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
 
     The operands come from the quantisers above.  Their rows may have any stride; the
     tensor-core kernels take operands whose rows start on 16-byte boundaries."""
-    if out is None and out_dtype not in (torch.bfloat16, torch.float32):
-        raise RuntimeError(f"gemm_s8: bf16 or fp32 output, not {out_dtype}")
     if _cuda(a):
         if out is None:
-            return torch.ops.harp.gemm_s8(a, a_scale, b, b_scale, bias, out_dtype == torch.float32,
+            return torch.ops.harp.gemm_s8(a, a_scale, b, b_scale, bias, _is_f32(out_dtype, "gemm_s8"),
                                           errors.word(a.device))
         torch.ops.harp.gemm_s8_out(a, a_scale, b, b_scale, bias, out, errors.word(a.device))
         return out
@@ -511,7 +516,7 @@ def gemm_s8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
     if bias is not None:
         acc = acc + bias.float()
     if out is None:
-        return acc.to(out_dtype)
+        return acc.float() if _is_f32(out_dtype, "gemm_s8") else acc.bfloat16()
     out.copy_(acc.to(out.dtype))
     return out
 
