@@ -756,10 +756,11 @@ long cluster_slots(int splits) {
 // measured on a B200: an SM takes in 135 KB a microsecond, all of them 14 MB; a pair
 // multiplies 256 x BN x 128 in 0.0014 BN; the epilogues take time by the columns a
 // CTA stores; a second wave of single-tile CTAs starts only when the first is done.
-// Of 44 shapes (M = 1 .. 17408, N = 24 .. 9216, K = 32 .. 6144) timed with every tile
-// and split, the choice was within 8 % of the fastest at 41 and within 20 % at all:
-// 4 x 1152 x 4608 takes 5.7 us with 8 splits and 10.8 with one; 1088 x 9216 x 1152 takes
-// 17.5 on CTA pairs and 30 in the rows kernel; 64 x 3456 x 1152 5.9 there and 6.7 on pairs.
+// Of 45 shapes (M = 1 .. 17408, N = 24 .. 9216, K = 32 .. 6144) timed with every tile
+// and split, weights in L2 and not, the choice was within 8 % of the fastest at 42 and
+// within 20 % at all: 4 x 1152 x 4608 takes 4.7 us with 8 splits and 9.5 with one; 4 x 6912 x
+// 1152 4.3 with one split and 8.1 with 4; 128 x 9216 x 1152 6.0 in the rows kernel and 6.4 on
+// CTA pairs; 1088 x 9216 x 1152 17.5 on CTA pairs and 30 in the rows kernel.
 struct Plan {
   int pair_bn;  // 256 / 192 / 128, or 0: the rows kernel with
   int nt, splits;
@@ -779,7 +780,7 @@ Plan pick(const S8Args& a) {
       const long slots = cluster_slots(sp);
       const long waves = (tiles * sp + slots - 1) / slots;
       const double one = 4.0 + (kb + sp - 1) / sp * load(tiles * sp, 16384 + 128 * nt) + 0.016 * nt +
-                         (sp == 1 ? 0.0 : sp == 2 ? 1.0 : 0.5);
+                         (sp == 1 ? 0.0 : sp <= 3 ? 1.0 : 0.5);
       const double t = 2.0 + waves * (one - 2.0);
       if (t < best_t) { best_t = t; best = {0, nt, sp}; }
     }

@@ -4,9 +4,10 @@
 
 Cases: gemm_qkv gemm_proj gemm_w13 gemm_w2 gemm_dw13 gemm_dx2 attn_fwd attn_bwd
 attn_fwd_d128 attn_bwd_d128 rmsnorm_fwd rmsnorm_bwd qknorm_fwd qknorm_bwd swiglu_fwd
-adamw (default: all).  Each case runs the harp kernel and, unless --no-ref,
-the library path of the same op (cuBLAS through torch.matmul, SDPA for
-attention).  Timing: CUDA events on the launching stream around each launch,
+adamw, and of int8 inference int8_qkv int8_w13 int8_w2 int8_ada int8_norm int8_swiglu
+int8_rows (default: all).  Each case runs the harp kernel and, unless --no-ref,
+the library path of the same op (cuBLAS through torch.matmul and torch._int_mm, SDPA
+for attention).  Timing: CUDA events on the launching stream around each launch,
 after 3 warm-up launches, with a 512 MiB write between timed launches so every
 launch starts from a cold L2 (126 MB).  Achieved TFLOP/s and GB/s are divided
 by MEASURED_PEAKS.json (copy bandwidth; cuBLAS bf16 burst) when present.
@@ -174,6 +175,32 @@ def adamw_case(n):
     return make
 
 
+def int8_gemm_case(M, N, K):
+    def make():
+        a, b = (torch.randint(-127, 128, (r, K), device="cuda", dtype=torch.int8) for r in (M, N))
+        sa, sb, bias = torch.rand(M, device="cuda"), torch.rand(N, device="cuda"), _r(N)
+        out = torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
+        harp = lambda: Fn.gemm_s8(a, sa, b, sb, bias=bias, out=out)  # noqa: E731
+        ref = (lambda: torch._int_mm(a, b.t())) if M > 16 else None  # the 32-bit sums alone
+        return harp, ref, {"flops": 2.0 * M * N * K, "shape": [M, N, K]}
+    return make
+
+
+def int8_rows_case(what: str):
+    def make():
+        R = B * S
+        x, res, mod = _r(R, D), _r(R, D), _r(B, 6 * D, scale=0.1)
+        if what == "swiglu":
+            gu = _r(R, 2 * F_)
+            return (lambda: Fn.swiglu_quant(gu, F_)), None, {"bytes": 5 * R * F_, "shape": [R, F_]}
+        if what == "rows":
+            return (lambda: Fn.quant_rows(x)), None, {"bytes": 3 * R * D, "shape": [R, D]}
+        harp = lambda: Fn.rmsnorm_mod_quant(x, None, mod[:, :D], mod[:, D:2 * D], S, 1e-6, residual=res,  # noqa: E731
+                                            gate=mod[:, 2 * D:3 * D])
+        return harp, None, {"bytes": 7 * R * D, "shape": [R, D]}
+    return make
+
+
 def build_cases(gemm_rows: int, adamw_n: int) -> Dict[str, Callable]:
     return {
         "gemm_qkv": gemm_case(gemm_rows, 3 * D, D),
@@ -193,6 +220,13 @@ def build_cases(gemm_rows: int, adamw_n: int) -> Dict[str, Callable]:
         "qknorm_bwd": qknorm_case(True),
         "swiglu_fwd": swiglu_case(),
         "adamw": adamw_case(adamw_n),
+        "int8_qkv": int8_gemm_case(gemm_rows, 3 * D, D),
+        "int8_w13": int8_gemm_case(gemm_rows, 2 * F_, D),
+        "int8_w2": int8_gemm_case(gemm_rows, D, F_),
+        "int8_ada": int8_gemm_case(B, 6 * D, D),
+        "int8_norm": int8_rows_case("norm"),
+        "int8_swiglu": int8_rows_case("swiglu"),
+        "int8_rows": int8_rows_case("rows"),
     }
 
 
