@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps) quant_rows_kernel(const QuantA
 // (a warp each, or the whole block for a wide row) go over the sample's rows with
 // the next row's loads under the reductions of this one.
 template <int MODE, typename T, int V, int N, bool MULTI>
-__global__ void __launch_bounds__(MULTI ? 32 * kMaxWarps : 128, MULTI ? 1 : MODE == kNormRes ? 3 : 4)
+__global__ void __launch_bounds__(MULTI ? 32 * kMaxWarps : 128, MULTI ? 1 : N > 5 && V == 8 ? 2 : MODE == kNormRes ? 3 : 4)
     norm_sample_kernel(const QuantArgs a, int warps) {
   constexpr bool TWO = MODE == kNormRes;
   constexpr int H = V == 8 ? 4 : V;  // a vector lies in V / H planes, so that wide reads meet no bank twice
@@ -721,6 +721,22 @@ void launch(const QuantArgs& a, cudaStream_t stream) {
     if constexpr (MODE >= kNorm) {
       const size_t smem = (size_t)groups * V * 4 * (MODE == kNormRes ? 3 : 2);
       by_sample = smem <= kVecSmem && a.R / a.rows_per_batch <= 65535 && a.rows_per_batch >= 8;
+      // A warp holds a row of up to 2560 values (its loads twice in fp32 with a residual: 1280). Wider
+      // rows take the block, at a barrier for each reduction: a weighted norm of 17408 x 2304 bf16 took
+      // 24.9 us on three warps a row, 19.2 on one; with a residual 4352 x 2560 17.9 and 14.2.
+      if constexpr (V == 8 && !(MODE == kNormRes && sizeof(T) == 4)) {
+        if (by_sample && groups > 160 && groups <= 320) {
+          switch ((groups + 31) / 32) {
+            case 6: launch_sample<MODE, T, 8, 6, false>(a, 1, smem, stream); break;
+            case 7: launch_sample<MODE, T, 8, 7, false>(a, 1, smem, stream); break;
+            case 8: launch_sample<MODE, T, 8, 8, false>(a, 1, smem, stream); break;
+            case 9: launch_sample<MODE, T, 8, 9, false>(a, 1, smem, stream); break;
+            default: launch_sample<MODE, T, 8, 10, false>(a, 1, smem, stream); break;
+          }
+          count_launch();
+          return;
+        }
+      }
       if (by_sample) {
 #define HARP_SAMPLE(V_, N_)                                                                 \
   (many.warps == 1 ? launch_sample<MODE, T, V_, N_, false>(a, many.warps, smem, stream)     \

@@ -106,7 +106,8 @@ class Int8Linear(nn.Module):
     def __init__(self, in_features, out_features, bias=True, device=None):
         super().__init__()
         self.in_features, self.out_features = in_features, out_features
-        self.register_buffer("weight_q", torch.zeros(out_features, in_features, device=device, dtype=torch.int8))
+        ld = -(-in_features // 16) * 16  # rows on 16-byte boundaries, as quant_rows lays them out
+        self.register_buffer("weight_q", torch.zeros(out_features, ld, device=device, dtype=torch.int8)[:, :in_features])
         self.register_buffer("weight_scale", torch.ones(out_features, device=device))
         self.register_buffer("bias", torch.zeros(out_features, device=device) if bias else None)
 

@@ -136,6 +136,44 @@ def test_rmsnorm_mod_quant(batch, rpb, cols, form, dt):
     _check_rows(q, s, y)
 
 
+WIDTHS = [1, 8, 56, 64, 72, 128, 130, 333, 334, 512, 1000, 1152, 1155, 1160, 1536, 1792, 2048, 2304, 2306, 2560, 2568,
+          3001, 4100, 4101, 4608, 6144, 7000, 8193, 12000]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("cols", WIDTHS)
+def test_many_rows(cols, dt):
+    """Enough rows for the kernels that take few warps a row and go over several rows."""
+    t, rpb, batch = DT[dt], 417, 3
+    R = rpb * batch
+    x, res = _x(R, cols, t, seed=6), _x(R, cols, t, seed=7)
+    q, s = Fn.quant_rows(x)
+    qc, sc = Fn.quant_rows(x.cpu())
+    assert torch.equal(q.cpu(), qc) and torch.equal(s.cpu(), sc)
+    gu = torch.cat([x, res], 1)
+    g, u = x.double(), res.double()
+    _check_rows(*Fn.swiglu_quant(gu, cols), g * torch.sigmoid(g) * u)
+    mod = _x(batch, 6 * cols, t, seed=8) * 0.1
+    scale, shift, gate = (mod[:, i * cols:(i + 1) * cols] for i in range(3))
+    w = _x(1, cols, t, seed=9)[0]
+    up = lambda v: v.double().repeat_interleave(rpb, 0)  # noqa: E731
+
+    def norm(h):
+        return h / torch.sqrt(h.pow(2).mean(1, keepdim=True) + 1e-6)
+
+    q, s, _ = Fn.rmsnorm_mod_quant(x, w, None, None, 0, 1e-6)
+    _check_rows(q, s, norm(x.double()) * w.double())
+    h64 = res.double() + up(gate) * x.double()
+    q, s, h = Fn.rmsnorm_mod_quant(x, w, scale, shift, rpb, 1e-6, residual=res, gate=gate)
+    _check_rows(q, s, norm(h64) * w.double() * (1 + up(scale)) + up(shift))
+    eps = 2.0 ** -8 if t == torch.bfloat16 else 2.0 ** -23
+    assert ((h.double() - h64).abs() <= eps * h64.abs() + 2.0 ** -22 * (res.double().abs() + (h64 - res.double()).abs())).all()
+    # samples of a few rows each
+    few = mod[:1].expand(R // 3, -1)[:, :cols]
+    q, s, h = Fn.rmsnorm_mod_quant(x, None, None, few, 3, 1e-6, residual=res)
+    _check_rows(q, s, norm(x.double() + res.double()) + mod[:1, :cols].double())
+
+
 def test_rows_special_values():
     """Zero rows, tiny rows, NaN and infinities: each row by itself."""
     x = torch.randn(8, 1152, generator=torch.Generator().manual_seed(0))
@@ -161,6 +199,12 @@ def test_rows_special_values():
         assert torch.isnan(Fn.dequant_rows(q, s)[r]).all()
     assert (q[6].abs() == 127).all() and torch.isfinite(s[6])
     assert q[7, 1151] == -127 and (q[7, :1151] == 0).all()
+    # many rows, a NaN in the modulation of one sample and in one row: nothing else is touched
+    y, m = torch.randn(1200, 1155, device="cuda"), torch.zeros(2, 1155, device="cuda")
+    m[1, 1154], y[5, 1154] = float("nan"), float("inf")
+    q, s, _ = Fn.rmsnorm_mod_quant(y, None, m, None, 600, 1e-6, residual=y, gate=m)
+    bad = torch.isnan(s)
+    assert bad[600:].all() and bad[5] and bad[:600].sum() == 1 and (q[bad] == 0).all()
     # norm: a zero row gives its shift; a NaN row stays its own
     z = torch.zeros(3, 64, device="cuda")
     z[1, 3] = float("nan")
