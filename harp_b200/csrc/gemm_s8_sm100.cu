@@ -8,7 +8,7 @@
 //
 // Three kernels:
 //   gemm_s8_pair  CTA pairs (cta_group::2), persistent over 256 x BN tiles: many
-//                 tokens and many channels.  Bound by the tensor pipe and, in a
+//                 tokens and many channels.  Bound by shared memory and, in a
 //                 long run, by power: 17408 x 9216 x 1152 in 138 to 165 us (2.7 to
 //                 2.2 PFLOP/s), 17408 x 1152 x 4608 in 69 to 82 us; run for a
 //                 second the GPU sits at its 1000 W and 1.37 GHz (zeros for operands:
@@ -116,6 +116,13 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 // of the next.  A stage is 256 deep in K (two 128-byte swizzle atoms a row), the
 // same bytes as the bf16 kernel's 128, at twice the arithmetic.  (Stages of 128 and
 // a commit for four MMAs instead of eight: 17408 x 1152 x 4608 in 101 us, not 83.)
+//
+// A 256 x 256 x 32 step takes 128 clocks, in which TMA writes 64 bytes a clock into
+// each SM's shared memory and the tensor core reads 64: all of its 128.  A tile of
+// K = 1152 therefore takes 4670 clocks (4608 of them MMA) without its epilogue and
+// 5813 with it, the difference being the block written to shared memory, read by the
+// TMA store, and the scales (1280 clocks of the same bandwidth).  It takes a larger
+// tile to move less, and two accumulators of 256 columns fill the tensor memory.
 //
 // Epilogue: each warp scales its 32 rows 128 bytes at a time, lays them out in
 // shared memory and one lane stores the block with TMA (whole 128-byte lines;
