@@ -6,8 +6,8 @@ Cases: gemm_qkv gemm_proj gemm_w13 gemm_w2 gemm_dw13 gemm_dx2 attn_fwd attn_bwd
 attn_fwd_d128 attn_bwd_d128 rmsnorm_fwd rmsnorm_bwd qknorm_fwd qknorm_bwd swiglu_fwd
 adamw, and of int8 inference int8_qkv int8_w13 int8_w2 int8_ada int8_norm int8_swiglu
 int8_rows (default: all).  Each case runs the harp kernel and, unless --no-ref,
-the library path of the same op (cuBLAS through torch.matmul and torch._int_mm, SDPA
-for attention).  Timing: CUDA events on the launching stream around each launch,
+the library path of the same op (cuBLAS through torch.matmul, SDPA for
+attention).  Timing: CUDA events on the launching stream around each launch,
 after 3 warm-up launches, with a 512 MiB write between timed launches so every
 launch starts from a cold L2 (126 MB).  Achieved TFLOP/s and GB/s are divided
 by MEASURED_PEAKS.json (copy bandwidth; cuBLAS bf16 burst) when present.
@@ -181,8 +181,7 @@ def int8_gemm_case(M, N, K):
         sa, sb, bias = torch.rand(M, device="cuda"), torch.rand(N, device="cuda"), _r(N)
         out = torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
         harp = lambda: Fn.gemm_s8(a, sa, b, sb, bias=bias, out=out)  # noqa: E731
-        ref = (lambda: torch._int_mm(a, b.t())) if M > 16 else None  # the 32-bit sums alone
-        return harp, ref, {"flops": 2.0 * M * N * K, "shape": [M, N, K]}
+        return harp, None, {"flops": 2.0 * M * N * K, "shape": [M, N, K]}
     return make
 
 
