@@ -472,3 +472,37 @@ def test_dependent_launches_are_ordered():
         graph.replay()
         assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
     errors.check(x0.device)
+
+
+def test_offsets_past_32_bits():
+    """Rows whose element offsets pass 2^31: the last ones against the same rows by themselves."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 40 << 30:
+        pytest.skip("needs 40 GB")
+    R, D = 2_097_400, 1032  # 2.16e9 values
+    x = torch.empty(R, D, dtype=torch.bfloat16, device="cuda")
+    tail = slice(R - 7, R)
+    x[: R - 7] = 1.0
+    x[tail] = _x(7, D, torch.bfloat16, seed=3)
+    q, s = Fn.quant_rows(x)
+    qt, st = Fn.quant_rows(x[tail])
+    assert torch.equal(q[tail], qt) and torch.equal(s[tail], st) and (q[:7] == 127).all() and (q[R // 2] == 127).all()
+    assert torch.equal(Fn.dequant_rows(q, s)[tail], Fn.dequant_rows(qt, st))
+    w = _x(1, D, torch.bfloat16, seed=4)[0]
+    q, s, h = Fn.rmsnorm_mod_quant(x, w, None, None, 0, 1e-6, residual=x)
+    y = x[tail].double() * 2
+    _check_rows(q[tail], s[tail], y / torch.sqrt(y.pow(2).mean(1, keepdim=True) + 1e-6) * w.double())
+    assert torch.equal(h[tail], (x[tail].float() * 2).bfloat16())
+    q, s = Fn.swiglu_quant(x, D // 2)
+    qt, st = Fn.swiglu_quant(x[tail], D // 2)
+    assert torch.equal(q[tail], qt) and torch.equal(s[tail], st)
+    del x, q, s, h
+    M, N = 240_000, 9216  # 2.2e9 results
+    a, b = _i8(M, 32, 1), _i8(N, 32, 2)
+    sa, sb = torch.rand(M, device="cuda"), torch.rand(N, device="cuda")
+    c = Fn.gemm_s8(a, sa, b, sb)
+    assert torch.equal(c[-9:], Fn.gemm_s8(a[-9:], sa[-9:], b, sb)) and torch.equal(c[:9], Fn.gemm_s8(a[:9], sa[:9], b, sb))
+    c = Fn.gemm_s8(a, sa, b[:1], sb[:1])  # one channel: the rows kernel or narrow pairs
+    ref = (a.double() @ b[:1].double().t()) * sa.double()[:, None] * sb[:1].double()
+    assert ((c.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 1e-30).all()
+    errors.check(a.device)
