@@ -6,7 +6,7 @@
 // result is one rounding of the sum to fp32, two products and an addition, and
 // does not depend on the order of the K loop, its split or the kernel chosen.
 //
-// Three kernels:
+// Two kernels:
 //   gemm_s8_pair  CTA pairs (cta_group::2), persistent over 256 x BN tiles: many
 //                 tokens and many channels.  Bound by shared memory and, in a
 //                 long run, by power: 17408 x 9216 x 1152 in 138 to 165 us (2.7 to
@@ -18,8 +18,7 @@
 //                 memory: few tokens (down to one) or few channels.  Bound by
 //                 latency: 4 x 6912 x 1152 4.5 to 5.9 us, 4 x 1152 x 4608 4.6 us back to
 //                 back, of which the weights' bytes are 1.2 and 0.8 us
-//   gemm_s8_simt  CUDA cores, for operands TMA cannot address (1061 x 1003 x 1155 with
-//                 odd row strides: 259 us, against 12 to 16 in the pair kernel)
+// Operands whose rows TMA cannot address are first copied to rows that it can.
 #include "common.cuh"
 #include "dependent_launch.cuh"
 #include "gemm_common.cuh"
@@ -49,7 +48,6 @@ struct S8Args {
   int bias_f32;
   void* C;
   long ldc;
-  int c_f32;
   int c_vec4;  // four neighbouring values of any row of C can be stored at once
   int* err;
 };
@@ -638,44 +636,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// CUDA-core kernel for operands TMA cannot address (rows that do not start on
-// 16-byte boundaries) and for K = 0.
-__global__ void __launch_bounds__(256) gemm_s8_simt(const S8Args a) {
-  __shared__ int As[32][33];
-  __shared__ int Bs[32][33];
-  dependency_release();
-  dependency_wait();
-  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;  // 32 x 8 threads
-  const int m0 = blockIdx.y * 32, n0 = blockIdx.x * 32;
-  int acc[4] = {0, 0, 0, 0};
-  for (int k0 = 0; k0 < a.K; k0 += 32) {
-    for (int r = ty; r < 32; r += 8) {
-      const int k = k0 + tx;
-      As[r][tx] = (m0 + r < a.M && k < a.K) ? (int)a.A[(long)(m0 + r) * a.lda + k] : 0;
-      Bs[r][tx] = (n0 + r < a.N && k < a.K) ? (int)a.B[(long)(n0 + r) * a.ldb + k] : 0;
-    }
-    __syncthreads();
-#pragma unroll 8
-    for (int kk = 0; kk < 32; ++kk) {
-      const int b = Bs[tx][kk];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] += As[ty + 8 * i][kk] * b;
-    }
-    __syncthreads();
-  }
-  const int n = n0 + tx;
-  if (n >= a.N) return;
-  const float sb = a.sb[n], bias = bias_at(a, n);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + ty + 8 * i;
-    if (m >= a.M) continue;
-    const float v = (float)acc[i] * a.sa[m] * sb + bias;
-    if (a.c_f32) reinterpret_cast<float*>(a.C)[(long)m * a.ldc + n] = v;
-    else reinterpret_cast<bf16*>(a.C)[(long)m * a.ldc + n] = __float2bfloat16(v);
-  }
-}
-
 // 2-D map over a row-major [rows, cols] matrix with row stride `ld_bytes`; box =
 // 128 bytes x box_rows, 128-byte swizzle.
 CUtensorMap make_map(const void* base, CUtensorMapDataType type, int esize, long rows, long cols, long ld_bytes,
@@ -828,6 +788,17 @@ void dispatch(const S8Args& a, bool c_tma, cudaStream_t stream) {
   }
 }
 
+// t, or a copy whose rows TMA can address: starting on 16-byte boundaries, not overlapping.
+at::Tensor addressable_rows(const at::Tensor& t) {
+  const int64_t rows = t.size(0), K = t.size(1);
+  if ((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 &&
+      (rows == 1 || (t.stride(0) % 16 == 0 && t.stride(0) >= K)))
+    return t;
+  at::Tensor c(at::detail::empty_strided_cuda({rows, K}, {(K + 15) / 16 * 16, 1}, at::kChar, t.device()));
+  c.copy_(t);
+  return c;
+}
+
 void check_scales(const at::Tensor& s, const at::Tensor& rows, const char* name) {
   TORCH_CHECK(s.is_cuda() && s.device() == rows.device() && s.scalar_type() == at::kFloat && s.dim() == 1 &&
                   s.size(0) == rows.size(0) && (s.size(0) <= 1 || s.stride(0) == 1),
@@ -862,40 +833,32 @@ void gemm_s8_out(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B,
   if (M == 0 || N == 0) return;
   const at::cuda::CUDAGuard guard(A.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  if (K == 0) {  // the sums are empty
+    auto none = at::outer(sa, sb).mul_(0);
+    C.copy_(bias.has_value() ? none.add_(*bias) : none);
+    return;
+  }
+  const at::Tensor Ar = addressable_rows(A), Br = addressable_rows(B);
   S8Args a = {};
   a.M = (int)M; a.N = (int)N; a.K = (int)K;
-  a.A = reinterpret_cast<const int8_t*>(A.data_ptr());
-  a.lda = A.stride(0);
-  a.B = reinterpret_cast<const int8_t*>(B.data_ptr());
-  a.ldb = B.stride(0);
+  a.A = reinterpret_cast<const int8_t*>(Ar.data_ptr());
+  a.B = reinterpret_cast<const int8_t*>(Br.data_ptr());
+  const long pad = (K + 15) / 16 * 16;  // a single row's stride is never used, but has to be valid
+  a.lda = M == 1 ? pad : Ar.stride(0);
+  a.ldb = N == 1 ? pad : Br.stride(0);
   a.sa = sa.data_ptr<float>();
   a.sb = sb.data_ptr<float>();
   a.bias = bias.has_value() ? bias->data_ptr() : nullptr;
   a.bias_f32 = bias.has_value() && bias->scalar_type() == at::kFloat;
   a.C = C.data_ptr();
   a.ldc = C.stride(0);
-  a.c_f32 = C.scalar_type() == at::kFloat;
   a.err = err.data_ptr<int>();
-  auto rows16 = [](const at::Tensor& t) {
-    return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 &&
-           (t.size(0) <= 1 || (t.stride(0) * t.element_size()) % 16 == 0);
-  };
-  // TMA: 16-byte aligned rows whose stride covers them (a stride of 0 or an overlap is left to the CUDA cores)
-  if (K > 0 && rows16(A) && rows16(B) && (M == 1 || a.lda >= K) && (N == 1 || a.ldb >= K)) {
-    const long pad = (K + 15) / 16 * 16;
-    if (M == 1) a.lda = pad;
-    if (N == 1) a.ldb = pad;
-    const bool c_tma = rows16(C) && (M == 1 || a.ldc >= N) && M > 1;
-    const uintptr_t where = reinterpret_cast<uintptr_t>(a.C) | (M == 1 ? 0 : (uintptr_t)(a.ldc * C.element_size()));
-    a.c_vec4 = where % (4 * C.element_size()) == 0;
-    if (a.c_f32) dispatch<float>(a, c_tma, stream);
-    else dispatch<bf16>(a, c_tma, stream);
-    return;
-  }
-  dim3 grid((unsigned)((N + 31) / 32), (unsigned)((M + 31) / 32));
-  TORCH_CHECK(grid.y <= 65535, "harp gemm_s8: too many rows for the CUDA-core path");
-  launch_dependent(gemm_s8_simt, grid, dim3(256), 0, stream, 1, a);
-  count_launch();
+  const uintptr_t where =
+      reinterpret_cast<uintptr_t>(a.C) | (M == 1 ? 0 : (uintptr_t)(a.ldc * (long)C.element_size()));
+  a.c_vec4 = where % (4 * C.element_size()) == 0;
+  const bool c_tma = where % 16 == 0 && M > 1 && a.ldc >= N;
+  if (C.scalar_type() == at::kFloat) dispatch<float>(a, c_tma, stream);
+  else dispatch<bf16>(a, c_tma, stream);
 }
 
 at::Tensor gemm_s8(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, const at::Tensor& sb,

@@ -499,8 +499,8 @@ def gemm_s8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
     """``(a @ b.T) * a_scale[:, None] * b_scale[None, :] + bias`` with ``a`` [M, K] and ``b`` [N, K]
     in int8 and exact 32-bit integer sums (K <= 131071); bf16 or fp32 result.
 
-    The operands come from the quantisers above.  Their rows may have any stride; the
-    tensor-core kernels take operands whose rows start on 16-byte boundaries."""
+    The operands come from the quantisers above, whose rows start on 16-byte boundaries.
+    Rows that do not are copied first."""
     if _cuda(a):
         if out is None:
             return torch.ops.harp.gemm_s8(a, a_scale, b, b_scale, bias, _is_f32(out_dtype, "gemm_s8"),
