@@ -442,6 +442,8 @@ def dequant_rows(q: torch.Tensor, s: torch.Tensor, dtype=torch.bfloat16) -> torc
     f32 = _is_f32(dtype, "dequant_rows")
     if _cuda(q):
         return torch.ops.harp.dequant_rows(q, s, f32)
+    if q.dtype != torch.int8 or q.dim() != 2 or s.shape != q.shape[:1] or s.dtype != torch.float32:
+        raise RuntimeError("dequant_rows: int8 rows [R, D] and an fp32 scale for each are required")
     return (q.float() * s[:, None]).to(dtype)
 
 
@@ -475,6 +477,14 @@ def rmsnorm_mod_quant(x: torch.Tensor, w: Optional[torch.Tensor], scale: Optiona
     _check_rows(x, "rmsnorm_mod_quant")
     if gate is not None and residual is None:
         raise RuntimeError("rmsnorm_mod_quant: gate needs a residual")
+    R, D = x.shape
+    for v in (scale, shift, gate):
+        if v is not None and (rows_per_batch < 1 or v.dtype != x.dtype or v.dim() != 2 or v.shape[1] != D
+                              or v.shape[0] * rows_per_batch != R):
+            raise RuntimeError("rmsnorm_mod_quant: scale, shift and gate must be [R / rows_per_batch, D] of x's type")
+    if (w is not None and (w.shape != (D,) or w.dtype != x.dtype)) or (
+            residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype)):
+        raise RuntimeError("rmsnorm_mod_quant: w must be [D] and residual [R, D], of x's type")
     xf = x.float()
     h = x
     if residual is not None:
@@ -509,6 +519,9 @@ def gemm_s8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
         return out
     if a.dtype != torch.int8 or b.dtype != torch.int8 or a.shape[1] != b.shape[1]:
         raise RuntimeError("gemm_s8: int8 operands [M, K] and [N, K] are required")
+    if a_scale.shape != a.shape[:1] or b_scale.shape != b.shape[:1] or (
+            bias is not None and bias.shape != b.shape[:1]):
+        raise RuntimeError("gemm_s8: a scale for each row of a and of b, and bias [N], are required")
     if a.shape[1] > 131071:
         raise RuntimeError(f"gemm_s8: K = {a.shape[1]} could overflow the 32-bit sums (at most 131071)")
     acc = (a.double() @ b.double().t()).float()  # the integer sum, exact in fp64

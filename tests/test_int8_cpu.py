@@ -79,7 +79,11 @@ def test_gemm_s8():
                 lambda: Fn.gemm_s8(a, sa, b, sb, out_dtype=torch.half), lambda: Fn.quant_rows(a.float()[0]),
                 lambda: Fn.quant_rows(a.half()), lambda: Fn.swiglu_quant(a.float(), 200),
                 lambda: Fn.rmsnorm_mod_quant(a.float(), None, None, None, 0, 1e-6, gate=a.float()),
-                lambda: Fn.dequant_rows(a, sa, torch.half)):
+                lambda: Fn.dequant_rows(a, sa, torch.half), lambda: Fn.dequant_rows(a, sa[:4]),
+                lambda: Fn.gemm_s8(a, sa[:1], b, sb), lambda: Fn.gemm_s8(a, sa, b, sb, bias=bias[:1]),
+                lambda: Fn.rmsnorm_mod_quant(a.float(), None, a[:1].float(), None, 3, 1e-6),
+                lambda: Fn.rmsnorm_mod_quant(a.float(), sa, None, None, 0, 1e-6),
+                lambda: Fn.rmsnorm_mod_quant(a.float(), None, None, None, 0, 1e-6, residual=b.float())):
         with pytest.raises(RuntimeError):
             bad()
 

@@ -506,3 +506,21 @@ def test_offsets_past_32_bits():
     ref = (a.double() @ b[:1].double().t()) * sa.double()[:, None] * sb[:1].double()
     assert ((c.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 1e-30).all()
     errors.check(a.device)
+
+
+def test_results_can_be_saved(tmp_path):
+    """What the quantisers return are tensors of their own: saved, loaded and copied like any."""
+    import copy
+
+    from harp_b200.ops.modules import Int8Linear, kpLinear
+
+    q, s = Fn.quant_rows(_x(5, 1155, torch.bfloat16))
+    torch.save({"q": q, "s": s}, tmp_path / "rows.pt")
+    d = torch.load(tmp_path / "rows.pt")
+    assert torch.equal(d["q"], q) and torch.equal(d["s"], s)
+    m = Int8Linear.from_linear(kpLinear(72, 40, dtype=torch.float32).cuda())
+    torch.save(m.state_dict(), tmp_path / "linear.pt")
+    n = Int8Linear(72, 40, device="cuda")
+    n.load_state_dict(torch.load(tmp_path / "linear.pt"))
+    x = _x(9, 72, torch.float32, seed=1)
+    assert torch.equal(m(x), n(x)) and torch.equal(m(x), copy.deepcopy(m)(x))
