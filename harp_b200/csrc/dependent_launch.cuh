@@ -13,6 +13,12 @@
 //
 // Every thread of a kernel launched so calls dependency_wait() before its first
 // access to global memory, also when it has nothing to do.
+//
+// What it then reads may have been written while it was already running, so it reads
+// with ordinary (coherent) loads, never through the read-only path, which wants data
+// that do not change during the kernel (and which the compiler may move ahead of the
+// wait): no read-only or cache-hint load intrinsics, no pointer parameters that promise
+// not to alias; loads in assembly are volatile.
 #pragma once
 
 #include <c10/cuda/CUDAException.h>

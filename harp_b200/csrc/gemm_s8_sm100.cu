@@ -332,12 +332,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       int mt, nt;
       pair_tile(t, num_m, num_n, args.N % BN != 0, mt, nt);
       const int m = mt * 256 + (int)rank * 128 + quarter * 32 + lane;
-      sa_next = m < args.M ? __ldg(args.sa + m) : 0.f;
+      sa_next = m < args.M ? args.sa[m] : 0.f;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int j = et + i * 128, n = nt * BN + j;
         const bool in = j < BN && n < args.N;
-        sb_next[i] = in ? __ldg(args.sb + n) : 0.f;
+        sb_next[i] = in ? args.sb[n] : 0.f;
         bias_next[i] = in ? bias_at(args, n) : 0.f;
       }
     };

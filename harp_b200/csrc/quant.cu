@@ -94,8 +94,32 @@ __device__ __forceinline__ Raw<V, T> load_raw(const T* p) {
   Raw<V, T> r;
   using E = std::remove_reference_t<decltype(r.v[0])>;
 #pragma unroll
-  for (int i = 0; i < (int)(sizeof(r.v) / sizeof(E)); ++i) r.v[i] = __ldg(reinterpret_cast<const E*>(p) + i);
+  for (int i = 0; i < (int)(sizeof(r.v) / sizeof(E)); ++i) r.v[i] = reinterpret_cast<const E*>(p)[i];
   return r;
+}
+// (volatile: a load in assembly stays behind dependency_wait() only so)
+__device__ __forceinline__ uint16_t ld_first(const uint16_t* p) {
+  uint16_t v;
+  asm volatile("ld.global.cs.u16 %0, [%1];" : "=h"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_first(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.global.cs.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 ld_first(const uint2* p) {
+  uint2 v;
+  asm volatile("ld.global.cs.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 ld_first(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
 }
 // Values of a row, which nothing reads again: first to leave the caches, so that
 // they do not push out what is being written (norm of 17408 x 1152 with a residual:
@@ -105,7 +129,7 @@ __device__ __forceinline__ Raw<V, T> load_once(const T* p) {
   Raw<V, T> r;
   using E = std::remove_reference_t<decltype(r.v[0])>;
 #pragma unroll
-  for (int i = 0; i < (int)(sizeof(r.v) / sizeof(E)); ++i) r.v[i] = __ldcs(reinterpret_cast<const E*>(p) + i);
+  for (int i = 0; i < (int)(sizeof(r.v) / sizeof(E)); ++i) r.v[i] = ld_first(reinterpret_cast<const E*>(p) + i);
   return r;
 }
 template <int V, typename T>
@@ -569,9 +593,8 @@ __global__ void __launch_bounds__(512) quant_wide_kernel(const QuantArgs a) {
 // q * s.  Rows of whole 16-byte groups: a thread turns 16 values of one row into
 // 32 (or 64) bytes; else neighbouring lanes take neighbouring values, V each.
 template <typename T>
-__global__ void __launch_bounds__(256) dequant_vec_kernel(const int8_t* __restrict__ q, long ldq,
-                                                          const float* __restrict__ s, long groups, int per_row,
-                                                          T* __restrict__ out) {
+__global__ void __launch_bounds__(256) dequant_vec_kernel(const int8_t* q, long ldq, const float* s, long groups,
+                                                          int per_row, T* out) {
   dependency_wait();
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= groups) return;
@@ -589,9 +612,8 @@ __global__ void __launch_bounds__(256) dequant_vec_kernel(const int8_t* __restri
   }
 }
 template <typename T, int V>
-__global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* __restrict__ q, long ldq,
-                                                           const float* __restrict__ s, long R, int D,
-                                                           T* __restrict__ out) {
+__global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* q, long ldq, const float* s, long R, int D,
+                                                           T* out) {
   dependency_wait();
   const long row = (long)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= R) return;
