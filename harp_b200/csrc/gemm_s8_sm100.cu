@@ -23,6 +23,7 @@
 #include "dependent_launch.cuh"
 #include "gemm_common.cuh"
 #include "gemm_sm100.h"
+#include "per_device.h"
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -677,10 +678,11 @@ int resident_clusters(void (*kern)(P...), int cluster, int smem) {
 }
 
 template <int BN, typename OUT>
-void launch_pair(const S8Args& a, bool c_tma, cudaStream_t stream) {
+void launch_pair(const S8Args& a, bool c_tma, int device, cudaStream_t stream) {
   using C_ = PairCfg<BN>;
   auto kern = gemm_s8_pair<BN, OUT>;
-  static const int max_clusters = resident_clusters(kern, 2, C_::SMEM_BYTES);
+  static PerDevice<int> clusters;
+  const int max_clusters = clusters.get(device, [&] { return resident_clusters(kern, 2, C_::SMEM_BYTES); });
   const CUtensorMap ta = make_map_s8(a.A, a.M, a.K, a.lda, 128), tb = make_map_s8(a.B, a.N, a.K, a.ldb, BN / 2);
   CUtensorMap tc = ta;
   if (c_tma)
@@ -694,12 +696,14 @@ void launch_pair(const S8Args& a, bool c_tma, cudaStream_t stream) {
 }
 
 template <int NT, typename OUT>
-void launch_rows(const S8Args& a, int splits, cudaStream_t stream) {
+void launch_rows(const S8Args& a, int splits, int device, cudaStream_t stream) {
   using C_ = RowsCfg<NT>;
   auto kern = gemm_s8_rows<NT, OUT>;
-  static const cudaError_t configured =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM_BYTES);
-  C10_CUDA_CHECK(configured);
+  static PerDevice<bool> configured;
+  configured.get(device, [&] {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM_BYTES));
+    return true;
+  });
   const CUtensorMap tw = make_map_s8(a.B, a.N, a.K, a.ldb, 128), tx = make_map_s8(a.A, a.M, a.K, a.lda, NT);
   const long ctas = (long)((a.N + 127) / 128) * ((a.M + NT - 1) / NT) * splits;
   TORCH_CHECK(ctas <= 0x7FFFFFFF, "harp gemm_s8: too many tiles");
@@ -709,15 +713,12 @@ void launch_rows(const S8Args& a, int splits, cudaStream_t stream) {
 
 // CTAs of the rows kernel that run at once in clusters of `splits` (larger clusters
 // leave SMs of a GPC over).
-long cluster_slots(int splits) {
-  static std::atomic<long> slots[9];
+long cluster_slots(int splits, int device) {
+  static PerDevice<long> slots[9];
   if (splits == 1) return num_sms();
-  long n = slots[splits].load(std::memory_order_relaxed);
-  if (n == 0) {
-    n = (long)splits * resident_clusters(gemm_s8_rows<16, bf16>, splits, RowsCfg<16>::SMEM_BYTES);
-    slots[splits].store(n, std::memory_order_relaxed);
-  }
-  return n;
+  return slots[splits].get(device, [&] {
+    return (long)splits * resident_clusters(gemm_s8_rows<16, bf16>, splits, RowsCfg<16>::SMEM_BYTES);
+  });
 }
 // The kernel and its tile by estimated time.  The constants are microseconds
 // measured on a B200: an SM takes in 135 KB a microsecond, all of them 14 MB; a pair
@@ -732,7 +733,7 @@ struct Plan {
   int pair_bn;  // 256 / 192 / 128, or 0: the rows kernel with
   int nt, splits;
 };
-Plan pick(const S8Args& a) {
+Plan pick(const S8Args& a, int device) {
   const int sms = num_sms();
   const long chans = (a.N + 127) / 128;
   const int kb = (a.K + 127) / 128;
@@ -744,7 +745,7 @@ Plan pick(const S8Args& a) {
   for (int nt : {16, 32, 64, 128, 256}) {
     const long tiles = chans * ((a.M + nt - 1) / nt);
     for (int sp = 1; sp <= 8 && sp <= kb; ++sp) {
-      const long slots = cluster_slots(sp);
+      const long slots = cluster_slots(sp, device);
       const long waves = (tiles * sp + slots - 1) / slots;
       const double one = 4.0 + (kb + sp - 1) / sp * load(tiles * sp, 16384 + 128 * nt) + 0.016 * nt +
                          (sp == 1 ? 0.0 : sp <= 3 ? 1.0 : 0.5);
@@ -763,28 +764,28 @@ Plan pick(const S8Args& a) {
 }
 
 template <typename OUT>
-void dispatch(const S8Args& a, bool c_tma, cudaStream_t stream) {
+void dispatch(const S8Args& a, bool c_tma, int device, cudaStream_t stream) {
   // the estimate takes about a microsecond on the host, so the plans of the sizes at hand are kept
   struct Known {
-    int M = -1, N = -1, K = -1;
+    int device = -1, M = -1, N = -1, K = -1;
     Plan p = {};
   };
   static thread_local Known known[64];
   Known& k = known[((unsigned)a.M * 7u + (unsigned)a.N * 31u + (unsigned)a.K * 131u) % 64u];
-  if (k.M != a.M || k.N != a.N || k.K != a.K) k = {a.M, a.N, a.K, pick(a)};
+  if (k.device != device || k.M != a.M || k.N != a.N || k.K != a.K) k = {device, a.M, a.N, a.K, pick(a, device)};
   const Plan p = k.p;
   switch (p.pair_bn) {
-    case 256: launch_pair<256, OUT>(a, c_tma, stream); return;
-    case 192: launch_pair<192, OUT>(a, c_tma, stream); return;
-    case 128: launch_pair<128, OUT>(a, c_tma, stream); return;
+    case 256: launch_pair<256, OUT>(a, c_tma, device, stream); return;
+    case 192: launch_pair<192, OUT>(a, c_tma, device, stream); return;
+    case 128: launch_pair<128, OUT>(a, c_tma, device, stream); return;
     default: break;
   }
   switch (p.nt) {
-    case 16: launch_rows<16, OUT>(a, p.splits, stream); break;
-    case 32: launch_rows<32, OUT>(a, p.splits, stream); break;
-    case 64: launch_rows<64, OUT>(a, p.splits, stream); break;
-    case 128: launch_rows<128, OUT>(a, p.splits, stream); break;
-    default: launch_rows<256, OUT>(a, p.splits, stream); break;
+    case 16: launch_rows<16, OUT>(a, p.splits, device, stream); break;
+    case 32: launch_rows<32, OUT>(a, p.splits, device, stream); break;
+    case 64: launch_rows<64, OUT>(a, p.splits, device, stream); break;
+    case 128: launch_rows<128, OUT>(a, p.splits, device, stream); break;
+    default: launch_rows<256, OUT>(a, p.splits, device, stream); break;
   }
 }
 
@@ -857,8 +858,8 @@ void gemm_s8_out(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B,
       reinterpret_cast<uintptr_t>(a.C) | (M == 1 ? 0 : (uintptr_t)(a.ldc * (long)C.element_size()));
   a.c_vec4 = where % (4 * C.element_size()) == 0;
   const bool c_tma = where % 16 == 0 && M > 1 && a.ldc >= N;
-  if (C.scalar_type() == at::kFloat) dispatch<float>(a, c_tma, stream);
-  else dispatch<bf16>(a, c_tma, stream);
+  if (C.scalar_type() == at::kFloat) dispatch<float>(a, c_tma, A.get_device(), stream);
+  else dispatch<bf16>(a, c_tma, A.get_device(), stream);
 }
 
 at::Tensor gemm_s8(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, const at::Tensor& sb,

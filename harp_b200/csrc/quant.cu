@@ -27,14 +27,13 @@
 #include "common.cuh"
 #include "dependent_launch.cuh"
 #include "gemm_sm100.h"
+#include "per_device.h"
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
-
-#include <mutex>
 
 namespace harp {
 
@@ -67,6 +66,7 @@ struct QuantArgs {
   int D;
   long rows_per_batch;
   float eps;
+  int device;  // that of every tensor here
 };
 
 __device__ __forceinline__ float to_f(float v) { return v; }
@@ -667,9 +667,10 @@ template <int MODE, typename T, int V, int N, bool MULTI>
 void launch_sample(const QuantArgs& a, int warps, size_t smem, cudaStream_t stream) {
   auto kern = norm_sample_kernel<MODE, T, V, N, MULTI>;
   const int threads = MULTI ? 32 * warps : 128, per_block = MULTI ? 1 : 4;
-  static std::once_flag once;
-  std::call_once(once, [&] {
+  static PerDevice<bool> configured;
+  configured.get(a.device, [&] {
     C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kVecSmem));
+    return true;
   });
   int n = 0;
   C10_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem));
@@ -828,6 +829,7 @@ void set_out(QuantArgs& a, const at::Tensor& q, const at::Tensor& s) {
   a.s = s.data_ptr<float>();
   a.R = q.size(0);
   a.D = (int)q.size(1);
+  a.device = q.get_device();
 }
 
 std::tuple<at::Tensor, at::Tensor> rows_or_swiglu(const at::Tensor& x, int64_t D, bool swiglu) {
