@@ -111,6 +111,17 @@ class Int8Linear(nn.Module):
         self.register_buffer("weight_scale", torch.ones(out_features, device=device))
         self.register_buffer("bias", torch.zeros(out_features, device=device) if bias else None)
 
+    def _apply(self, fn, *args, **kwargs):
+        """Moves and conversions of the module: the scales stay in fp32, as they are the weights' own, and the
+        bias in a type that the product adds (bf16 or fp32)."""
+        was = {n: getattr(self, n) for n in ("weight_scale", "bias")}
+        super()._apply(fn, *args, **kwargs)
+        for n, types in (("weight_scale", (torch.float32,)), ("bias", (torch.float32, torch.bfloat16))):
+            t = getattr(self, n)
+            if t is not None and t.dtype not in types:
+                setattr(self, n, was[n].to(t.device))
+        return self
+
     @classmethod
     @torch.no_grad()
     def from_weight(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "Int8Linear":

@@ -1,0 +1,33 @@
+"""Int8Linear as a module: conversions, moves and inputs that any linear layer takes."""
+import pytest
+import torch
+
+from harp_b200.ops import functional as Fn
+from harp_b200.ops.modules import Int8Linear, kpLinear
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _layer(i=100, o=40, bias=True, device="cpu"):
+    torch.manual_seed(0)
+    return Int8Linear.from_linear(kpLinear(i, o, bias=bias, dtype=torch.float32).to(device))
+
+
+def _x(*shape, dtype=torch.float32, device="cpu"):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(1)).to(device, dtype)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("how", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(),
+                                 lambda m: m.bfloat16().float(), lambda m: torch.nn.Sequential(m).half()[0]])
+@pytest.mark.parametrize("bias", [True, False])
+def test_dtype_conversions_keep_the_scales(device, how, bias):
+    m, x = _layer(bias=bias, device=device), _x(7, 100, device=device)
+    scale, y = m.weight_scale.clone(), m(x)
+    m = how(m)
+    assert m.weight_q.dtype == torch.int8 and m.weight_scale.dtype == torch.float32
+    assert torch.equal(m.weight_scale, scale) and m.weight_scale.device == x.device
+    assert not bias or m.bias.dtype in (torch.bfloat16, torch.float32)
+    # at most the bias is rounded, once, to bf16's 8 bits
+    b = m.bias.float() if bias else torch.zeros(())
+    assert ((m(x) - y).abs() <= 2.0 ** -8 * b.abs().to(x.device) + 2.0 ** -22 * y.abs()).all()
