@@ -97,6 +97,14 @@ def replace_linear_with_kplinear(model: nn.Module, kplinear_class=kpLinear) -> n
     return model
 
 
+def _rows16(q: torch.Tensor) -> torch.Tensor:
+    """int8 rows [N, K] on 16-byte boundaries, which the int8 product reads in place: q, or a copy."""
+    if q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.stride(0) >= q.shape[1]:
+        return q
+    out = q.new_zeros(q.shape[0], -(-q.shape[1] // 16) * 16)[:, :q.shape[1]]
+    return out.copy_(q)
+
+
 class Int8Linear(nn.Module):
     """Inference linear layer in 8-bit integers: the weight [out, in] in int8 with a scale
     for each output channel, the input quantised per row (``functional.quant_rows``), the
@@ -106,27 +114,28 @@ class Int8Linear(nn.Module):
     def __init__(self, in_features, out_features, bias=True, device=None):
         super().__init__()
         self.in_features, self.out_features = in_features, out_features
-        ld = -(-in_features // 16) * 16  # rows on 16-byte boundaries, as quant_rows lays them out
-        self.register_buffer("weight_q", torch.zeros(out_features, ld, device=device, dtype=torch.int8)[:, :in_features])
+        self.register_buffer("weight_q", _rows16(torch.zeros(out_features, in_features, device=device, dtype=torch.int8)))
         self.register_buffer("weight_scale", torch.ones(out_features, device=device))
         self.register_buffer("bias", torch.zeros(out_features, device=device) if bias else None)
 
     def _apply(self, fn, *args, **kwargs):
-        """Moves and conversions of the module: the scales stay in fp32, as they are the weights' own, and the
-        bias in a type that the product adds (bf16 or fp32)."""
+        """Moves and conversions of the module: the scales stay in fp32, as they are the weights' own, the
+        bias in a type that the product adds (bf16 or fp32), and the weight's rows on their boundaries."""
         was = {n: getattr(self, n) for n in ("weight_scale", "bias")}
         super()._apply(fn, *args, **kwargs)
         for n, types in (("weight_scale", (torch.float32,)), ("bias", (torch.float32, torch.bfloat16))):
             t = getattr(self, n)
             if t is not None and t.dtype not in types:
                 setattr(self, n, was[n].to(t.device))
+        self.weight_q = _rows16(self.weight_q)
         return self
 
     @classmethod
     @torch.no_grad()
     def from_weight(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "Int8Linear":
         m = cls(weight.shape[1], weight.shape[0], bias=False, device="meta")
-        m.weight_q, m.weight_scale = Fn.quant_rows(weight.detach())
+        q, m.weight_scale = Fn.quant_rows(weight.detach())
+        m.weight_q = _rows16(q)
         m.bias = bias.detach().clone() if bias is not None else None
         return m
 

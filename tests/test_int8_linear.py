@@ -31,3 +31,28 @@ def test_dtype_conversions_keep_the_scales(device, how, bias):
     # at most the bias is rounded, once, to bf16's 8 bits
     b = m.bias.float() if bias else torch.zeros(())
     assert ((m(x) - y).abs() <= 2.0 ** -8 * b.abs().to(x.device) + 2.0 ** -22 * y.abs()).all()
+
+
+def _padded(q):
+    return q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.data_ptr() % 16 == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("i", [1, 100, 1155, 64])
+def test_rows_stay_on_16_byte_boundaries(device, i):
+    """What the int8 product reads in place: a layer that is built on the CPU, moved or copied keeps its rows there."""
+    import copy
+
+    m, x = _layer(i), _x(3, i)
+    y = m(x)
+    assert _padded(m.weight_q)
+    w = m.weight_q.clone()
+    for move in (lambda m: m.to(device), lambda m: m.cpu().to(device), copy.deepcopy, lambda m: m.to(torch.bfloat16)):
+        m = move(m)
+        assert m.weight_q.shape == (40, i) and _padded(m.weight_q) and torch.equal(m.weight_q.cpu(), w)
+    m = m.to("meta").to_empty(device=device)
+    assert m.weight_q.shape == (40, i) and _padded(m.weight_q)
+    m = Int8Linear(i, 40)
+    m.load_state_dict(_layer(i).state_dict())
+    assert _padded(m.weight_q) and torch.equal(m(x), y)
+    assert _padded(m.to(device).weight_q)
