@@ -105,6 +105,11 @@ def _rows16(q: torch.Tensor) -> torch.Tensor:
     return out.copy_(q)
 
 
+def _unit_inner(x: torch.Tensor) -> torch.Tensor:
+    """x with neighbouring values next to each other, as the quantisers read a row: x, or a copy."""
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
 class Int8Linear(nn.Module):
     """Inference linear layer in 8-bit integers: the weight [out, in] in int8 with a scale
     for each output channel, the input quantised per row (``functional.quant_rows``), the
@@ -134,7 +139,7 @@ class Int8Linear(nn.Module):
     @torch.no_grad()
     def from_weight(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "Int8Linear":
         m = cls(weight.shape[1], weight.shape[0], bias=False, device="meta")
-        q, m.weight_scale = Fn.quant_rows(weight.detach())
+        q, m.weight_scale = Fn.quant_rows(_unit_inner(weight.detach()))
         m.weight_q = _rows16(q)
         m.bias = bias.detach().clone() if bias is not None else None
         return m
@@ -154,7 +159,7 @@ class Int8Linear(nn.Module):
 
     @torch.no_grad()
     def forward(self, x):
-        q, s = Fn.quant_rows(x.reshape(-1, x.shape[-1]))
+        q, s = Fn.quant_rows(_unit_inner(x.reshape(-1, x.shape[-1])))
         return self.rows(q, s, x.dtype).view(*x.shape[:-1], self.out_features)
 
 

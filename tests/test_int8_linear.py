@@ -56,3 +56,17 @@ def test_rows_stay_on_16_byte_boundaries(device, i):
     m.load_state_dict(_layer(i).state_dict())
     assert _padded(m.weight_q) and torch.equal(m(x), y)
     assert _padded(m.to(device).weight_q)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_inputs_and_weights_of_any_stride(device):
+    """A transposed view as input (one sample of [B, C, L] seen as [B, L, C], a transposed matrix) or as weight."""
+    m = _layer(100, 40, device=device)
+    for x in (_x(1, 100, 6, device=device).transpose(1, 2), _x(100, 6, device=device).t(),
+              _x(2, 100, 6, device=device).transpose(1, 2), _x(5, 200, device=device)[:, ::2],
+              _x(6, 1, device=device).expand(6, 100)):
+        assert torch.equal(m(x), m(x.contiguous()))
+    w = _x(100, 40, device=device)
+    n = Int8Linear.from_weight(w.t())
+    ref = Int8Linear.from_weight(w.t().contiguous())
+    assert torch.equal(n.weight_q, ref.weight_q) and torch.equal(n.weight_scale, ref.weight_scale)
