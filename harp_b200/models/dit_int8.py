@@ -40,8 +40,8 @@ class DiTInt8Block(nn.Module):
         self.proj = Int8Linear.from_weight(proj_w, proj_b)
         self.w13 = Int8Linear.from_weight(_w13(w1, w3), None)
         self.w2 = Int8Linear.from_weight(w2, w2_b)
-        self.register_buffer("q_norm", qn_w.detach() if qn_w is not None else None)
-        self.register_buffer("k_norm", kn_w.detach() if kn_w is not None else None)
+        self.register_buffer("q_norm", qn_w.detach().clone() if qn_w is not None else None)
+        self.register_buffer("k_norm", kn_w.detach().clone() if kn_w is not None else None)
 
     def forward(self, a: torch.Tensor, x: Optional[torch.Tensor], gate: Optional[torch.Tensor], c8, freqs, B: int, S: int,
                 sp: SPContext) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:

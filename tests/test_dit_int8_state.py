@@ -1,0 +1,36 @@
+"""What the int8 DiT holds of the model it was built from."""
+import torch
+
+from harp_b200.models.dit import DiT, DiTConfig
+
+CFG = DiTConfig(in_channels=4, hidden=96, depth=2, heads=2, mlp_ratio=4.0, text_dim=64, axes_dims=(16, 16, 16))
+
+
+def _model():
+    torch.manual_seed(0)
+    m = DiT(CFG)
+    with torch.no_grad():
+        for n, p in m.named_parameters():
+            p.normal_(0, 0.02 if "adaLN" in n else 0.08)
+            if "norm" in n:
+                p.add_(1.0)
+    return m.bfloat16()
+
+
+def _inputs():
+    g = torch.Generator().manual_seed(1)
+    return (torch.randn(2, 4, 8, 8, generator=g).bfloat16(), torch.randn(2, 16, 64, generator=g).bfloat16(),
+            torch.tensor([0.3, 0.8]))
+
+
+def test_the_blocks_hold_nothing_of_the_model_they_were_built_from():
+    """A step that changes the model's blocks afterwards changes nothing in the int8 ones."""
+    m = _model()
+    q = m.int8()
+    theirs = {p.untyped_storage().data_ptr() for p in m.blocks.parameters()}
+    assert not [n for n, b in q.blocks.named_buffers() if b.untyped_storage().data_ptr() in theirs]
+    before = q(*_inputs())
+    with torch.no_grad():
+        for p in m.blocks.parameters():
+            p.mul_(-3.0).add_(0.5)
+    assert torch.equal(q(*_inputs()), before)
