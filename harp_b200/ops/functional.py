@@ -419,9 +419,19 @@ def _is_f32(dtype: torch.dtype, op: str) -> bool:
     raise RuntimeError(f"{op}: bf16 or fp32 output, not {dtype}")
 
 
+# The CPU statements refuse what the kernels refuse, so that what runs here runs there.
+def _unit_inner(x: torch.Tensor) -> bool:
+    return x.shape[1] <= 1 or x.stride(1) == 1
+
+
 def _check_rows(x: torch.Tensor, op: str) -> None:
-    if x.dtype not in (torch.bfloat16, torch.float32) or x.dim() != 2 or x.shape[1] < 1:
-        raise RuntimeError(f"{op}: a 2-D bf16 or fp32 tensor with at least one column is required")
+    if x.dtype not in (torch.bfloat16, torch.float32) or x.dim() != 2 or not 1 <= x.shape[1] <= 1 << 30 or (
+            not _unit_inner(x)):
+        raise RuntimeError(f"{op}: a 2-D bf16 or fp32 tensor with 1 to 2^30 columns and a unit inner stride is required")
+
+
+def _is_vector(v: torch.Tensor, n: int, *types: torch.dtype) -> bool:
+    return v.dim() == 1 and v.shape[0] == n and v.dtype in types and (n <= 1 or v.stride(0) == 1)
 
 
 def quant_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -442,8 +452,8 @@ def dequant_rows(q: torch.Tensor, s: torch.Tensor, dtype=torch.bfloat16) -> torc
     f32 = _is_f32(dtype, "dequant_rows")
     if _cuda(q):
         return torch.ops.harp.dequant_rows(q, s, f32)
-    if q.dtype != torch.int8 or q.dim() != 2 or s.shape != q.shape[:1] or s.dtype != torch.float32:
-        raise RuntimeError("dequant_rows: int8 rows [R, D] and an fp32 scale for each are required")
+    if q.dtype != torch.int8 or q.dim() != 2 or not _unit_inner(q) or not _is_vector(s, q.shape[0], torch.float32):
+        raise RuntimeError("dequant_rows: int8 rows [R, D] of unit inner stride and a dense fp32 scale for each are required")
     return (q.float() * s[:, None]).to(dtype)
 
 
@@ -480,11 +490,13 @@ def rmsnorm_mod_quant(x: torch.Tensor, w: Optional[torch.Tensor], scale: Optiona
     R, D = x.shape
     for v in (scale, shift, gate):
         if v is not None and (rows_per_batch < 1 or v.dtype != x.dtype or v.dim() != 2 or v.shape[1] != D
-                              or v.shape[0] * rows_per_batch != R):
-            raise RuntimeError("rmsnorm_mod_quant: scale, shift and gate must be [R / rows_per_batch, D] of x's type")
-    if (w is not None and (w.shape != (D,) or w.dtype != x.dtype)) or (
-            residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype)):
-        raise RuntimeError("rmsnorm_mod_quant: w must be [D] and residual [R, D], of x's type")
+                              or v.shape[0] * rows_per_batch != R or not _unit_inner(v)):
+            raise RuntimeError("rmsnorm_mod_quant: scale, shift and gate must be [R / rows_per_batch, D] of x's type "
+                               "with a unit inner stride")
+    if (w is not None and not _is_vector(w, D, x.dtype)) or (
+            residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype
+                                      or not _unit_inner(residual))):
+        raise RuntimeError("rmsnorm_mod_quant: w must be a dense [D] and residual [R, D] with a unit inner stride, of x's type")
     xf = x.float()
     h = x
     if residual is not None:
@@ -517,13 +529,19 @@ def gemm_s8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
                                           errors.word(a.device))
         torch.ops.harp.gemm_s8_out(a, a_scale, b, b_scale, bias, out, errors.word(a.device))
         return out
-    if a.dtype != torch.int8 or b.dtype != torch.int8 or a.shape[1] != b.shape[1]:
-        raise RuntimeError("gemm_s8: int8 operands [M, K] and [N, K] are required")
-    if a_scale.shape != a.shape[:1] or b_scale.shape != b.shape[:1] or (
-            bias is not None and bias.shape != b.shape[:1]):
-        raise RuntimeError("gemm_s8: a scale for each row of a and of b, and bias [N], are required")
+    if a.dtype != torch.int8 or b.dtype != torch.int8 or a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[1] or (
+            not _unit_inner(a) or not _unit_inner(b)):
+        raise RuntimeError("gemm_s8: int8 operands [M, K] and [N, K] of unit inner stride are required")
+    M, N = a.shape[0], b.shape[0]
+    if not _is_vector(a_scale, M, torch.float32) or not _is_vector(b_scale, N, torch.float32):
+        raise RuntimeError("gemm_s8: dense fp32 scales, one for each row of a and of b, are required")
+    if bias is not None and not _is_vector(bias, N, torch.float32, torch.bfloat16):
+        raise RuntimeError(f"gemm_s8: bias must be a dense bf16 or fp32 vector of {N} values")
     if a.shape[1] > 131071:
         raise RuntimeError(f"gemm_s8: K = {a.shape[1]} could overflow the 32-bit sums (at most 131071)")
+    if out is not None and (out.shape != (M, N) or out.dtype not in (torch.float32, torch.bfloat16)
+                            or not _unit_inner(out)):
+        raise RuntimeError(f"gemm_s8: out must be [{M}, {N}] in bf16 or fp32 with a unit inner stride")
     acc = (a.double() @ b.double().t()).float()  # the integer sum, exact in fp64
     acc = acc * a_scale[:, None] * b_scale[None, :]
     if bias is not None:
