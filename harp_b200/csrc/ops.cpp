@@ -297,6 +297,12 @@ TORCH_LIBRARY_IMPL(harp, CUDA, m) {
   m.impl("gemm_s8_out", &harp::gemm_s8_out);
 }
 
+// No gradient passes a rounding to 8 bits: results of these carry none, whatever the operands carry.
+TORCH_LIBRARY_IMPL(harp, Autograd, m) {
+  for (const char* op : {"quant_rows", "swiglu_quant", "rmsnorm_mod_quant", "dequant_rows", "gemm_s8", "gemm_s8_out"})
+    m.impl(op, torch::CppFunction::makeFallthrough());
+}
+
 TORCH_LIBRARY_IMPL(harp, CompositeExplicitAutograd, m) {
   m.impl("launch_count", &harp::launch_count_op);
   m.impl("add_launch_count", &harp::add_launch_count_op);

@@ -397,12 +397,14 @@ def gate_bwd(dy, a, gate, rows_per_batch, want_bias=True):
 
 
 # ---------------------------------------------------------------------------
-# 8-bit integer rows and their GEMM (inference: no gradient passes the rounding)
+# 8-bit integer rows and their GEMM (inference: no gradient passes the rounding, so
+# the results carry none, whatever the operands carry)
 # ---------------------------------------------------------------------------
 _INT8_MIN_SCALE = 2.0 ** -126
 
 
 def _rows8(y: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    y = y.detach()
     amax = y.abs().amax(1)
     s = (amax * (1.0 / 127.0)).clamp_min(_INT8_MIN_SCALE)
     q = torch.round(y * (1.0 / s)[:, None])
@@ -454,7 +456,7 @@ def dequant_rows(q: torch.Tensor, s: torch.Tensor, dtype=torch.bfloat16) -> torc
         return torch.ops.harp.dequant_rows(q, s, f32)
     if q.dtype != torch.int8 or q.dim() != 2 or not _unit_inner(q) or not _is_vector(s, q.shape[0], torch.float32):
         raise RuntimeError("dequant_rows: int8 rows [R, D] of unit inner stride and a dense fp32 scale for each are required")
-    return (q.float() * s[:, None]).to(dtype)
+    return (q.float() * s.detach()[:, None]).to(dtype)
 
 
 def swiglu_quant(gu: torch.Tensor, F_: int) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -502,7 +504,7 @@ def rmsnorm_mod_quant(x: torch.Tensor, w: Optional[torch.Tensor], scale: Optiona
     if residual is not None:
         if gate is not None:
             xf = _bcast(gate.float(), rows_per_batch) * xf
-        xf = residual.float() + xf
+        xf = (residual.float() + xf).detach()
         h = xf.to(x.dtype)
     y = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
     if w is not None:
@@ -546,6 +548,7 @@ def gemm_s8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
     acc = acc * a_scale[:, None] * b_scale[None, :]
     if bias is not None:
         acc = acc + bias.float()
+    acc = acc.detach()
     if out is None:
         return acc.float() if _is_f32(out_dtype, "gemm_s8") else acc.bfloat16()
     out.copy_(acc.to(out.dtype))
