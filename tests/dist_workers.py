@@ -570,3 +570,16 @@ def zimage_reference_sp(rank, world, out, args):
     (pred_o.float() * w[:, lo:hi]).sum().backward()
     res.update(pred_ours=pred_o.detach().float(), range=(lo, hi), grads_ours=grads(ours))
     return res
+
+
+def dit_int8_sp(rank, world, out, args):
+    """The int8 DiT's sequence-parallel forward: this rank's predictions and their range of image tokens."""
+    from harp_b200.parallel.sequence import SPContext
+    from test_dit_int8_state import _inputs, _model
+
+    q = _model().int8()
+    lat, text, t = _inputs()
+    sp = SPContext.from_group(dist.group.WORLD, backend="torch", mode=args["mode"])
+    n = lat.shape[-1] // q.cfg.patch_size
+    pred, lo, hi = q.forward_local(q.patchify(lat), text, t, n, n, sp)
+    return {"pred": pred, "lo": lo, "hi": hi}

@@ -1,4 +1,5 @@
-"""What the int8 DiT holds of the model it was built from."""
+"""What the int8 DiT holds of the model it was built from, and its sequence-parallel forward."""
+import pytest
 import torch
 
 from harp_b200.models.dit import DiT, DiTConfig
@@ -34,3 +35,27 @@ def test_the_blocks_hold_nothing_of_the_model_they_were_built_from():
         for p in m.blocks.parameters():
             p.mul_(-3.0).add_(0.5)
     assert torch.equal(q(*_inputs()), before)
+
+
+@pytest.mark.timeout(600)
+@pytest.mark.parametrize("world,mode", [(2, "ring"), (2, "ulysses"), (4, "ring")])
+def test_sequence_parallel_forward(world, mode, tmp_path):
+    """Rows are quantised each by itself, so ranks differ from one process only by the attention's order of sums,
+    bf16's 8 bits and the 8-bit values that this moves to a neighbour (as the CUDA form from the CPU one)."""
+    from test_dist_gloo import _run
+
+    from harp_b200.parallel.sequence import SPContext
+
+    q = _model().int8()
+    lat, text, t = _inputs()
+    n = lat.shape[-1] // q.cfg.patch_size
+    ref = q.forward_local(q.patchify(lat), text, t, n, n, SPContext.single())[0].float()
+    res = _run("dit_int8_sp", world, tmp_path, {"mode": mode})[0]
+    seen = 0
+    for r in range(world):
+        lo, hi, pred = res[r]["lo"], res[r]["hi"], res[r]["pred"].float()
+        assert lo == min(seen, ref.shape[1]) and pred.shape[1] == hi - lo and not res[r]["pred"].requires_grad
+        seen = hi
+        if hi > lo:
+            assert ((pred - ref[:, lo:hi]).norm() / ref[:, lo:hi].norm()).item() < 3e-2
+    assert seen == ref.shape[1]
