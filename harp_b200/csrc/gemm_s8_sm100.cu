@@ -125,8 +125,9 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 //
 // Epilogue: each warp scales its 32 rows 128 bytes at a time, lays them out in
 // shared memory and one lane stores the block with TMA (whole 128-byte lines;
-// out of range rows and columns are dropped by the map).  A C that TMA cannot
-// address is written from the same buffer, a row of the block at a time.  Stored
+// out of range rows and 16-byte groups are dropped by the map).  A C that TMA cannot
+// address, or whose rows end inside a group, is written from the same buffer, a row of
+// the block at a time.  Stored
 // straight from registers, 32 bytes a lane, 17408 x 9216 x 1152 took 187 us, not 154;
 // eight epilogue warps instead of four changed nothing (190 and 187 at that time).
 // ---------------------------------------------------------------------------
@@ -857,7 +858,8 @@ void gemm_s8_out(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B,
   const uintptr_t where =
       reinterpret_cast<uintptr_t>(a.C) | (M == 1 ? 0 : (uintptr_t)(a.ldc * (long)C.element_size()));
   a.c_vec4 = where % (4 * C.element_size()) == 0;
-  const bool c_tma = where % 16 == 0 && M > 1 && a.ldc >= N;
+  // TMA stores whole 16-byte groups: past a width that ends inside one it would overwrite what lies beside C
+  const bool c_tma = where % 16 == 0 && N * C.element_size() % 16 == 0 && M > 1 && a.ldc >= N;
   if (C.scalar_type() == at::kFloat) dispatch<float>(a, c_tma, A.get_device(), stream);
   else dispatch<bf16>(a, c_tma, A.get_device(), stream);
 }
