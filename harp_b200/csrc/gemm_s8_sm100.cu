@@ -37,6 +37,9 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 
+constexpr int64_t kMostRows = 0x7FFFFF00;  // of either operand
+constexpr int64_t kMostK = 131071;
+
 struct S8Args {
   int M, N, K;
   const int8_t* A;
@@ -764,9 +767,8 @@ Plan pick(const S8Args& a, int device) {
   return best;
 }
 
-template <typename OUT>
-void dispatch(const S8Args& a, bool c_tma, int device, cudaStream_t stream) {
-  // the estimate takes about a microsecond on the host, so the plans of the sizes at hand are kept
+// pick(), with the plans of the sizes at hand kept: the estimate takes about a microsecond on the host.
+Plan plan_of(const S8Args& a, int device) {
   struct Known {
     int device = -1, M = -1, N = -1, K = -1;
     Plan p = {};
@@ -774,7 +776,12 @@ void dispatch(const S8Args& a, bool c_tma, int device, cudaStream_t stream) {
   static thread_local Known known[64];
   Known& k = known[((unsigned)a.M * 7u + (unsigned)a.N * 31u + (unsigned)a.K * 131u) % 64u];
   if (k.device != device || k.M != a.M || k.N != a.N || k.K != a.K) k = {device, a.M, a.N, a.K, pick(a, device)};
-  const Plan p = k.p;
+  return k.p;
+}
+
+template <typename OUT>
+void dispatch(const S8Args& a, bool c_tma, int device, cudaStream_t stream) {
+  const Plan p = plan_of(a, device);
   switch (p.pair_bn) {
     case 256: launch_pair<256, OUT>(a, c_tma, device, stream); return;
     case 192: launch_pair<192, OUT>(a, c_tma, device, stream); return;
@@ -819,8 +826,8 @@ void gemm_s8_out(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B,
   const int64_t M = A.size(0), N = B.size(0), K = A.size(1);
   TORCH_CHECK(B.size(1) == K, "harp gemm_s8: A has ", std::to_string(K), " columns and B ", std::to_string(B.size(1)));
   TORCH_CHECK(C.size(0) == M && C.size(1) == N, "harp gemm_s8: C shape");
-  TORCH_CHECK(K <= 131071, "harp gemm_s8: K = ", std::to_string(K), " could overflow the 32-bit sums (at most 131071)");
-  TORCH_CHECK(M <= 0x7FFFFF00 && N <= 0x7FFFFF00, "harp gemm_s8: M and N below 2^31");
+  TORCH_CHECK(K <= kMostK, "harp gemm_s8: K = ", std::to_string(K), " could overflow the 32-bit sums (at most 131071)");
+  TORCH_CHECK(M <= kMostRows && N <= kMostRows, "harp gemm_s8: M and N below 2^31");
   TORCH_CHECK((A.stride(1) == 1 || K <= 1) && (B.stride(1) == 1 || K <= 1) && (C.stride(1) == 1 || N <= 1),
               "harp gemm_s8: unit inner stride");
   TORCH_CHECK(C.scalar_type() == at::kBFloat16 || C.scalar_type() == at::kFloat, "harp gemm_s8: bf16 or fp32 output");
@@ -870,6 +877,18 @@ at::Tensor gemm_s8(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& 
   at::Tensor C(at::detail::empty_cuda({A.size(0), B.size(0)}, f32 ? at::kFloat : at::kBFloat16, A.device(), c10::nullopt));
   gemm_s8_out(A, sa, B, sb, bias, C, err);
   return C;
+}
+
+// The kernel that a product of these sizes runs on the current device: (pair tile's columns, 0, 0) or
+// (0, tokens a CTA, splits of K).
+std::tuple<int64_t, int64_t, int64_t> gemm_s8_plan(int64_t M, int64_t N, int64_t K) {
+  TORCH_CHECK(M >= 1 && M <= kMostRows && N >= 1 && N <= kMostRows && K >= 1 && K <= kMostK,
+              "harp gemm_s8: no plan for these sizes");
+  S8Args a = {};
+  a.M = (int)M; a.N = (int)N; a.K = (int)K;
+  const Plan p = plan_of(a, at::cuda::current_device());
+  if (p.pair_bn != 0) return {p.pair_bn, 0, 0};
+  return {0, p.nt, p.splits};
 }
 
 }  // namespace harp

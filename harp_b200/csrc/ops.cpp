@@ -70,6 +70,7 @@ at::Tensor gemm_s8(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& 
                    const c10::optional<at::Tensor>& bias, bool f32, at::Tensor err);
 void gemm_s8_out(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, const at::Tensor& sb,
                  const c10::optional<at::Tensor>& bias, at::Tensor C, at::Tensor err);
+std::tuple<int64_t, int64_t, int64_t> gemm_s8_plan(int64_t M, int64_t N, int64_t K);
 
 namespace {
 
@@ -261,6 +262,7 @@ TORCH_LIBRARY(harp, m) {
   m.def("dequant_rows(Tensor q, Tensor s, bool f32) -> Tensor");
   m.def("gemm_s8(Tensor A, Tensor sa, Tensor B, Tensor sb, Tensor? bias, bool f32, Tensor(a!) err) -> Tensor");
   m.def("gemm_s8_out(Tensor A, Tensor sa, Tensor B, Tensor sb, Tensor? bias, Tensor(a!) C, Tensor(b!) err) -> ()");
+  m.def("gemm_s8_plan(int M, int N, int K) -> (int, int, int)");
   m.def("launch_count() -> int");
   m.def("add_launch_count(int n) -> ()");
   m.def("reset_launch_count() -> ()");
@@ -304,6 +306,7 @@ TORCH_LIBRARY_IMPL(harp, Autograd, m) {
 }
 
 TORCH_LIBRARY_IMPL(harp, CompositeExplicitAutograd, m) {
+  m.impl("gemm_s8_plan", &harp::gemm_s8_plan);
   m.impl("launch_count", &harp::launch_count_op);
   m.impl("add_launch_count", &harp::add_launch_count_op);
   m.impl("reset_launch_count", &harp::reset_launch_count_op);
