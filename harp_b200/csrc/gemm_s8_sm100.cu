@@ -830,6 +830,7 @@ void gemm_s8_out(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B,
   TORCH_CHECK(M <= kMostRows && N <= kMostRows, "harp gemm_s8: M and N below 2^31");
   TORCH_CHECK((A.stride(1) == 1 || K <= 1) && (B.stride(1) == 1 || K <= 1) && (C.stride(1) == 1 || N <= 1),
               "harp gemm_s8: unit inner stride");
+  TORCH_CHECK(M <= 1 || C.stride(0) >= N, "harp gemm_s8: rows of C overlap");
   TORCH_CHECK(C.scalar_type() == at::kBFloat16 || C.scalar_type() == at::kFloat, "harp gemm_s8: bf16 or fp32 output");
   TORCH_CHECK(err.scalar_type() == at::kInt && err.numel() >= 4, "harp gemm_s8: error word");
   check_scales(sa, A, "a_scale");
@@ -866,7 +867,7 @@ void gemm_s8_out(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B,
       reinterpret_cast<uintptr_t>(a.C) | (M == 1 ? 0 : (uintptr_t)(a.ldc * (long)C.element_size()));
   a.c_vec4 = where % (4 * C.element_size()) == 0;
   // TMA stores whole 16-byte groups: past a width that ends inside one it would overwrite what lies beside C
-  const bool c_tma = where % 16 == 0 && N * C.element_size() % 16 == 0 && M > 1 && a.ldc >= N;
+  const bool c_tma = where % 16 == 0 && N * C.element_size() % 16 == 0 && M > 1;
   if (C.scalar_type() == at::kFloat) dispatch<float>(a, c_tma, A.get_device(), stream);
   else dispatch<bf16>(a, c_tma, A.get_device(), stream);
 }

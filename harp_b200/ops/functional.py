@@ -542,8 +542,9 @@ def gemm_s8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
     if a.shape[1] > 131071:
         raise RuntimeError(f"gemm_s8: K = {a.shape[1]} could overflow the 32-bit sums (at most 131071)")
     if out is not None and (out.shape != (M, N) or out.dtype not in (torch.float32, torch.bfloat16)
-                            or not _unit_inner(out)):
-        raise RuntimeError(f"gemm_s8: out must be [{M}, {N}] in bf16 or fp32 with a unit inner stride")
+                            or not _unit_inner(out) or (M > 1 and out.stride(0) < N)):
+        raise RuntimeError(f"gemm_s8: out must be [{M}, {N}] in bf16 or fp32 with a unit inner stride and rows that do "
+                           "not overlap")
     acc = (a.double() @ b.double().t()).float()  # the integer sum, exact in fp64
     acc = acc * a_scale[:, None] * b_scale[None, :]
     if bias is not None:

@@ -78,6 +78,11 @@ REFUSED = {
     "gemm out rows": lambda i8, s, **k: Fn.gemm_s8(i8[:1], s[:1], i8, s, out=torch.empty(4, 4, device=i8.device)),
     "gemm out columns": lambda i8, s, **k: Fn.gemm_s8(i8, s, i8[:1], s[:1], out=torch.empty(4, 4, device=i8.device)),
     "gemm out transposed": lambda i8, s, **k: Fn.gemm_s8(i8, s, i8[:3], s[:3], out=torch.empty(3, 4, device=i8.device).t()),
+    "gemm out of one row repeated": lambda i8, s, **k: Fn.gemm_s8(i8, s, i8, s, out=torch.empty(1, 4, device=i8.device).expand(4, 4)),
+    "gemm out with overlapping rows": lambda i8, s, **k: Fn.gemm_s8(i8, s, i8, s, out=torch.empty(16, device=i8.device).as_strided(
+        (4, 4), (3, 1))),
+    "gemm out of one column repeated": lambda i8, s, **k: Fn.gemm_s8(i8, s, i8[:1], s[:1], out=torch.empty(
+        1, device=i8.device).as_strided((4, 1), (0, 1))),
     "gemm 1-D out": lambda i8, s, **k: Fn.gemm_s8(i8[:1], s[:1], i8, s, out=torch.empty(4, device=i8.device)),
 }
 
@@ -90,6 +95,8 @@ TAKEN = {
     "bf16 bias, fp32 output": lambda i8, s, **k: Fn.gemm_s8(i8, s, i8, s, bias=s.bfloat16(), out_dtype=torch.float32),
     "fp32 bias, bf16 output": lambda i8, s, **k: Fn.gemm_s8(i8, s, i8, s, bias=s),
     "output in a wider matrix": lambda i8, s, wide, **k: Fn.gemm_s8(i8, s, i8, s, out=wide[:, 9:13]),
+    "output of one row": lambda i8, s, **k: Fn.gemm_s8(i8[:1], s[:1], i8, s, out=torch.empty(1, 4, device=i8.device).as_strided((1, 4), (2, 1))),
+    "output of every second row": lambda i8, s, wide, **k: Fn.gemm_s8(i8[:2], s[:2], i8, s, out=wide[::2, :4]),
     "K of zero": lambda i8, s, **k: Fn.gemm_s8(i8[:, :0], s, i8[:, :0], s, bias=s),
 }
 
