@@ -8,17 +8,17 @@
 //
 // Two kernels:
 //   gemm_s8_pair  CTA pairs (cta_group::2), persistent over 256 x BN tiles: many
-//                 tokens and many channels.  Bound by shared memory and, in a
-//                 long run, by power: 17408 x 9216 x 1152 in 138 to 165 us (2.7 to
-//                 2.2 PFLOP/s), 17408 x 1152 x 4608 in 69 to 82 us; run for a
-//                 second the GPU sits at its 1000 W and 1.37 GHz (zeros for operands:
-//                 119 us at 1.97 GHz)
+//                 tokens and many channels.  17408 x 9216 x 1152 in 137 us alone
+//                 (2.7 PFLOP/s) and 161 us run for seconds, where the GPU sits at its
+//                 1000 W and 1.31 GHz (zeros for operands: 117 us at 1.97 GHz);
+//                 17408 x 1152 x 4608 in 68 to 73 us alone and 80 us run for seconds
 //   gemm_s8_rows  128 channels x up to 256 tokens a CTA, the K loop split over a
 //                 cluster that adds its integer sums through distributed shared
 //                 memory: few tokens (down to one) or few channels.  Bound by
-//                 latency: 4 x 6912 x 1152 4.5 to 5.9 us, 4 x 1152 x 4608 4.6 us back to
+//                 latency: 4 x 6912 x 1152 in 4.4 us and 4 x 1152 x 4608 in 4.7 us back to
 //                 back, of which the weights' bytes are 1.2 and 0.8 us
-// Operands whose rows TMA cannot address are first copied to rows that it can.
+// Operands whose rows TMA cannot address are first copied to rows that it can
+// (1061 x 1003 x 1155 in 19 us, 12 without the copies).
 #include "common.cuh"
 #include "dependent_launch.cuh"
 #include "gemm_common.cuh"
@@ -119,12 +119,17 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 // same bytes as the bf16 kernel's 128, at twice the arithmetic.  (Stages of 128 and
 // a commit for four MMAs instead of eight: 17408 x 1152 x 4608 in 101 us, not 83.)
 //
-// A 256 x 256 x 32 step takes 128 clocks, in which TMA writes 64 bytes a clock into
-// each SM's shared memory and the tensor core reads 64: all of its 128.  A tile of
-// K = 1152 therefore takes 4670 clocks (4608 of them MMA) without its epilogue and
-// 5813 with it, the difference being the block written to shared memory, read by the
-// TMA store, and the scales (1280 clocks of the same bandwidth).  It takes a larger
-// tile to move less, and two accumulators of 256 columns fill the tensor memory.
+// What bounds it: a 256 x 256 tile of K = 1152 is 36 steps of 128 clocks, 4608 in all.
+// The 2448 tiles of 17408 x 9216 x 1152 are 34 rounds of the 74 pairs that are resident
+// (the last of 6 tiles).  A round takes 5160 clocks of the SMs and 0.81 us that do not
+// shrink with their clock: fitted, within 1 %, to runs of a second and more at 1312 MHz
+// (161.3 us, 991 W), 1417 MHz (operands of -1 .. 1: 152.4 us) and 1965 MHz (zeros:
+// 116.9 us).  So in a long run power sets the clock, and at full clock a quarter of a
+// round is time outside the SMs, whose operands arrive at 12.4 TB/s from L2.  In the same
+// way 17408 x 1152 x 4608 takes 100400 clocks, 82900 of them MMAs of the busiest pair
+// (four whole tiles and a narrow one), and 7.6 us.  Fewer operand bytes would help
+// against both: a row band's A kept in shared memory over its column tiles, where K lets it
+// fit, and half the B for a narrow band, which is loaded whole.
 //
 // Epilogue: each warp scales its 32 rows 128 bytes at a time, lays them out in
 // shared memory and one lane stores the block with TMA (whole 128-byte lines;
@@ -732,7 +737,9 @@ long cluster_slots(int splits, int device) {
 // and split, weights in L2 and not, the choice was within 8 % of the fastest at 42 and
 // within 20 % at all: 4 x 1152 x 4608 takes 4.7 us with 8 splits and 9.5 with one; 4 x 6912 x
 // 1152 4.3 with one split and 8.1 with 4; 128 x 9216 x 1152 6.0 in the rows kernel and 6.4 on
-// CTA pairs; 1088 x 9216 x 1152 17.5 on CTA pairs and 30 in the rows kernel.
+// CTA pairs; 1088 x 9216 x 1152 14.6 to 17.5 on CTA pairs and 30 in the rows kernel.  It does not
+// know of outputs that TMA cannot store: 1061 x 1003 x 1155 into such rows of fp32 takes 12 us, 1061 x
+// 1008 x 1155 7.7.
 struct Plan {
   int pair_bn;  // 256 / 192 / 128, or 0: the rows kernel with
   int nt, splits;

@@ -17,13 +17,14 @@
 // NaN, as it is in bf16.
 //
 // Bound by memory: each value is read once and held in registers between the
-// row's reductions and the rounding.  Measured on one B200 (inputs and outputs over
-// the kernel's time; 6.5 TB/s is a copy), bf16: quant_rows of 17408 x 1152 10.3 us
-// (5.8 TB/s), swiglu_quant of 17408 x 4608 66 us (6.0), rmsnorm_mod_quant of 17408 x
-// 1152 with residual, gate and modulation 20.4 us (6.9, part of it from L2), dequant_rows
-// of 17408 x 1152 10.9 us (5.5); one to a few hundred rows take 2 to 3 us, launch included.
-// Widths that are not multiples of 8 read 2 or 1 values at a time: 17408 x 1154 22 us,
-// 17408 x 1155 31 us (bound by instructions).
+// row's reductions and the rounding.  Measured on one B200, bf16, on three sets of inputs
+// in turn, of which L2 (126 MB) still holds a part, and in brackets after 512 MB were
+// written: quant_rows of 17408 x 1152 9.8 us (16.4), swiglu_quant of 17408 x 4608 66.7 us
+// (71.7), rmsnorm_mod_quant of 17408 x 1152 with residual, gate and modulation 20.3 us
+// (31.7), dequant_rows of 17408 x 1152 10.9 us (16.4); a copy of the same bytes at 6.5 TB/s
+// takes 9.2, 61.3, 21.5 and 9.2.  One to a few hundred rows take 1.3 to 2.1 us back to back.
+// Widths that are not multiples of 8 read 2 or 1 values at a time: 17408 x 1154 21.4 us
+// (28.7), 17408 x 1155 31.2 us (38.9), bound by instructions.
 #include "common.cuh"
 #include "dependent_launch.cuh"
 #include "gemm_sm100.h"
@@ -123,7 +124,7 @@ __device__ __forceinline__ uint4 ld_first(const uint4* p) {
 }
 // Values of a row, which nothing reads again: first to leave the caches, so that
 // they do not push out what is being written (norm of 17408 x 1152 with a residual:
-// 25.9 us, 30.6 without).
+// 25.9 us, 30.6 without, when this was added).
 template <int V, typename T>
 __device__ __forceinline__ Raw<V, T> load_once(const T* p) {
   Raw<V, T> r;

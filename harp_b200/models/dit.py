@@ -476,7 +476,8 @@ class DiT(nn.Module):
 
     def int8(self) -> "DiTInt8":
         """This model for inference with its blocks' products in 8-bit integers
-        (harp_b200.models.dit_int8); embedders and final layer are shared."""
+        (harp_b200.models.dit_int8); embedders and final layer are shared, the blocks are
+        copied as they are now."""
         from .dit_int8 import DiTInt8
 
         return DiTInt8(self)

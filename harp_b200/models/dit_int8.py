@@ -62,7 +62,7 @@ class DiTInt8Block(nn.Module):
 
 class DiTInt8(DiT):
     """A DiT whose blocks multiply in int8.  Built from a DiT in bf16; the DiT's embedders and
-    final layer are used as they are, its blocks' weights are read once and not kept."""
+    final layer are used as they are, its blocks are read once and nothing of them is kept."""
 
     def __init__(self, model: DiT):
         nn.Module.__init__(self)

@@ -521,7 +521,8 @@ def gemm_s8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
             bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
             out_dtype=torch.bfloat16) -> torch.Tensor:
     """``(a @ b.T) * a_scale[:, None] * b_scale[None, :] + bias`` with ``a`` [M, K] and ``b`` [N, K]
-    in int8 and exact 32-bit integer sums (K <= 131071); bf16 or fp32 result.
+    in int8 and exact 32-bit integer sums (K <= 131071); bf16 or fp32 result, in ``out`` if given (which
+    may be part of a wider matrix).
 
     The operands come from the quantisers above, whose rows start on 16-byte boundaries.
     Rows that do not are copied first."""

@@ -7,7 +7,7 @@ attn_fwd_d128 attn_bwd_d128 rmsnorm_fwd rmsnorm_bwd qknorm_fwd qknorm_bwd swiglu
 adamw, and of int8 inference int8_qkv int8_w13 int8_w2 int8_ada int8_norm int8_swiglu
 int8_rows (default: all).  Each case runs the harp kernel and, unless --no-ref,
 the library path of the same op (cuBLAS through torch.matmul, SDPA for
-attention).  Timing: CUDA events on the launching stream around each launch,
+attention; the int8 cases have none).  Timing: CUDA events on the launching stream around each launch,
 after 3 warm-up launches, with a 512 MiB write between timed launches so every
 launch starts from a cold L2 (126 MB).  Achieved TFLOP/s and GB/s are divided
 by MEASURED_PEAKS.json (copy bandwidth; cuBLAS bf16 burst) when present.
