@@ -59,3 +59,25 @@ def test_sequence_parallel_forward(world, mode, tmp_path):
         if hi > lo:
             assert ((pred - ref[:, lo:hi]).norm() / ref[:, lo:hi].norm()).item() < 3e-2
     assert seen == ref.shape[1]
+
+
+@pytest.mark.gpu
+def test_a_model_quantised_on_the_cpu_and_moved():
+    """The quantisers give the same bits on both sides, so where the weights were quantised makes no difference."""
+    import copy
+
+    from harp_b200.models import dit as D
+
+    torch.manual_seed(0)
+    m = D.DiT(D.PRESETS["small"])
+    with torch.no_grad():
+        for n, p in m.named_parameters():
+            p.normal_(0, 0.02 if "adaLN" in n else 0.05)
+    m = m.bfloat16()
+    a, b = m.int8().cuda().to(torch.bfloat16), copy.deepcopy(m).cuda().int8()
+    for (n, p), (_, q) in zip(a.named_buffers(), b.named_buffers()):
+        assert torch.equal(p, q) and p.stride() == q.stride() and p.dtype == q.dtype, n
+    g = torch.Generator().manual_seed(1)
+    x = (torch.randn(2, 16, 16, 16, generator=g).bfloat16().cuda(), torch.randn(2, 32, 384, generator=g).bfloat16().cuda(),
+         torch.rand(2, generator=g).cuda())
+    assert torch.equal(a(*x), b(*x))
